@@ -1429,9 +1429,18 @@ ARGMAX_CHUNK = 2048
 
 
 def sample(logits: torch.Tensor, temperature: Optional[torch.Tensor] = None,
-           uniform: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+           uniform: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, top_k: Optional[torch.Tensor] = None,
+           top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One token per row of float32 logits: argmax where the row's temperature
-    is 0 (or none is given), else a draw with the row's uniform number."""
+    is 0 (or none is given), else a draw with the row's uniform number.
+
+    ``top_k`` (int32 [rows]; <= 0 or >= the vocabulary: off), ``top_p`` and ``min_p`` (float32 [rows]; >= 1 and <= 0: off) are the
+    rules that each row's draw is under.  A token weighs ``w = exp((l - max l) / T)``, NaN and -inf nothing.  Kept are the first
+    ``top_k`` tokens (the larger logit first, of equal ones the lower index), of these the ones in front of which less than
+    ``top_p`` of their weight lies (the first always), and of these the ones with ``w >= min_p`` (the largest always).  The token
+    is the first kept one by index whose running sum of ``w`` passes ``uniform`` times the kept ones' sum."""
+    if not (top_k is None and top_p is None and min_p is None):
+        return _sample_rules(logits, temperature, uniform, out, top_k, top_p, min_p)
     _gpu("logits", logits, torch.float32, 2)
     rows, vocab = logits.shape
     if temperature is None and vocab >= 4 * ARGMAX_CHUNK:
@@ -1467,6 +1476,126 @@ def sample(logits: torch.Tensor, temperature: Optional[torch.Tensor] = None,
         return out
     _run("cie_sample", load_library().cie_sample(_stream(), _ptr(logits), _ptr(temperature), _ptr(uniform),
                                                  _ptr(out), _i(rows), _i(vocab), _i(vocab)))
+    return out
+
+
+def _on_current_gpu(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    """All operands on the GPU whose stream the kernel will run on."""
+    index = first.get_device()
+    if index != torch._C._cuda_getDevice():
+        raise ValueError(f"the operands live on {first.device}, and cuda:{torch._C._cuda_getDevice()} is the current device")
+    for other in others:
+        if other is not None and other.get_device() != index:
+            raise ValueError(f"operands on {first.device} and {other.device}")
+
+
+def _logit_rows(logits: torch.Tensor) -> tuple[int, int]:
+    """Float32 rows on the GPU, each in one piece (they may lie apart)."""
+    _row_view("logits", logits, tuple(logits.shape), (torch.float32,))
+    rows, vocab = logits.shape
+    if vocab < 1:
+        raise ValueError(f"logits of shape {tuple(logits.shape)}")
+    return rows, vocab
+
+
+def _per_row(name: str, t: torch.Tensor, dtype: torch.dtype, rows: int) -> None:
+    _gpu(name, t, dtype, 1)
+    if t.shape[0] != rows:
+        raise ValueError(f"{name} must be [{rows}], is {list(t.shape)}")
+
+
+MAX_RULE_ROWS = 65535
+
+
+def _sample_rules(logits, temperature, uniform, out, top_k, top_p, min_p) -> torch.Tensor:
+    rows, vocab = _logit_rows(logits)
+    if temperature is None or uniform is None:
+        raise ValueError("a draw under rules needs temperatures and uniform numbers")
+    if rows > MAX_RULE_ROWS:
+        raise ValueError(f"up to {MAX_RULE_ROWS} rows, not {rows}")
+    _per_row("temperature", temperature, torch.float32, rows)
+    _per_row("uniform", uniform, torch.float32, rows)
+    for name, rule, dtype in (("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if rule is not None:
+            _per_row(name, rule, dtype, rows)
+    if out is None:
+        out = torch.empty((rows,), dtype=torch.int32, device=logits.device)
+    _per_row("out", out, torch.int32, rows)
+    _on_current_gpu(logits, temperature, uniform, top_k, top_p, min_p, out)
+    if rows == 0:
+        return out
+    _run("cie_sample_rules", load_library().cie_sample_rules(
+        _stream(), _ptr(logits), _ptr(temperature), _ptr(uniform), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(out), _i(rows),
+        _i(vocab), _i(_ld(logits))))
+    return out
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """What the rows of float32 logits give their tokens (int32 [rows]): ``(l_t - max l) - log sum_i exp(l_i - max l)``, float32
+    [rows].  The rows of ``logits`` may lie apart.  A token outside the vocabulary gives NaN, and so does a row with a NaN, a
+    +inf, or nothing but -inf."""
+    rows, vocab = _logit_rows(logits)
+    _per_row("tokens", tokens, torch.int32, rows)
+    if out is None:
+        out = torch.empty((rows,), dtype=torch.float32, device=logits.device)
+    _per_row("out", out, torch.float32, rows)
+    _on_current_gpu(logits, tokens, out)
+    if rows == 0:
+        return out
+    _run("cie_token_logprobs", load_library().cie_token_logprobs(_stream(), _ptr(logits), _ptr(tokens), _ptr(out), _i(rows),
+                                                                _i(vocab), _i(_ld(logits))))
+    return out
+
+
+# ---------------------------------------------------------------------------
+MAX_ADAPTER_RANK = 128
+MAX_ADAPTER_PIECES = 4
+
+
+def lora_add(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale: torch.Tensor, adapters: torch.Tensor,
+             into: torch.Tensor, columns: Optional[tuple] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``out[t] = into[t] + scale[a] * up[a] @ (down[a] @ x[t])`` with ``a = adapters[t]``: every row's own low-rank adapter beside
+    a product that all rows share.  A row whose adapter is negative (or not below ``A``) keeps its numbers.
+
+    x [T, K]; down [A, P * R, K]; up [A, N, R]; scale float32 [A]; adapters int32 [T]; into [T, N] in x's type or float32 (the
+    residual stream).  ``columns``: the widths of the P projections that are stacked in the N columns (default: one); projection p
+    reads rows p R .. (p + 1) R of ``down``.  ``out`` (default: ``into`` itself) is of into's type.  x, into and out may be views
+    whose rows lie apart; out is ``into`` or shares nothing with any operand.  Sums are float32, rounded once.  A row's result
+    does not depend on the other rows."""
+    if x.dim() != 2 or into.dim() != 2:
+        raise ValueError(f"x {tuple(x.shape)} and into {tuple(into.shape)} must be matrices")
+    rows, k = x.shape
+    n = into.shape[1]
+    code = _code(x.dtype)
+    _row_view("x", x, (rows, k), (x.dtype,))
+    _row_view("into", into, (rows, n), (x.dtype, torch.float32))
+    columns = (n,) if columns is None else tuple(columns)
+    pieces = len(columns)
+    if not 1 <= pieces <= MAX_ADAPTER_PIECES or min(columns) < 1 or sum(columns) != n:
+        raise ValueError(f"columns {columns} must be 1 to {MAX_ADAPTER_PIECES} positive widths that add up to {n}")
+    _gpu("down", down, x.dtype, 3)
+    _gpu("up", up, x.dtype, 3)
+    count, n_up, rank = up.shape
+    if not (1 <= rank <= MAX_ADAPTER_RANK and n_up == n and tuple(down.shape) == (count, pieces * rank, k) and count >= 1 and k >= 1):
+        raise ValueError(f"down {tuple(down.shape)} and up {tuple(up.shape)} do not fit rows of {k}, {n} columns in {pieces} pieces "
+                         f"and a rank of 1 to {MAX_ADAPTER_RANK}")
+    _per_row("scale", scale, torch.float32, count)
+    _per_row("adapters", adapters, torch.int32, rows)
+    if out is None:
+        out = into
+    else:
+        _row_view("out", out, (rows, n), (into.dtype,))
+    _on_current_gpu(x, down, up, scale, adapters, into, out)
+    if rows > 65535:
+        raise ValueError(f"up to 65,535 rows, not {rows}")
+    if rows == 0:
+        return out
+    inner = torch.empty(rows * pieces * rank, dtype=torch.float32, device=x.device)
+    begins = [sum(columns[:p]) for p in range(1, pieces)] + [n] * (MAX_ADAPTER_PIECES - pieces)
+    _run("cie_lora_add", load_library().cie_lora_add(
+        _stream(), _i(code), _i(_code(into.dtype)), _ptr(x), _i(_ld(x)), _ptr(down), _ptr(up), _ptr(scale), _ptr(adapters),
+        _ptr(into), _i(_ld(into)), _ptr(out), _i(_ld(out)), _ptr(inner), _i(rows), _i(k), _i(n), _i(rank), _i(count), _i(pieces),
+        _i(begins[0]), _i(begins[1]), _i(begins[2])))
     return out
 
 

@@ -1,0 +1,212 @@
+"""GPU: low-rank adapters of many requests beside a shared projection, against their definition in 64 bits."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from cie_amd.kernels import ops
+
+    return ops
+
+
+def site(rows, k, columns, rank, count, dtype, stream=False, seed=0, adapters=None):
+    """x, down, up, scale, adapters, into on the CPU, with odd values everywhere."""
+    g = torch.Generator().manual_seed(seed)
+    n, parts = sum(columns), len(columns)
+    if adapters is None:
+        adapters = torch.randint(-1, count, (rows,), generator=g)
+    return dict(
+        x=torch.randn((rows, k), generator=g).to(dtype), down=(torch.randn((count, parts * rank, k), generator=g) * k ** -0.5).to(dtype),
+        up=(torch.randn((count, n, rank), generator=g) * rank ** -0.5).to(dtype), scale=torch.rand(count, generator=g) + 0.5,
+        adapters=torch.as_tensor(adapters, dtype=torch.int32),
+        into=torch.randn((rows, n), generator=g).to(torch.float32 if stream else dtype), columns=tuple(columns))
+
+
+def definition(s):
+    """The result in 64 bits, and how far a right kernel may be from it.
+
+    A sum of n products in float32, in any order, is off by at most n 2^-24 of the sum of their sizes; the inner products may
+    be held as two bfloat16 numbers (2^-17 of their size) on their way into the second one; then the scale, the addition and
+    the rounding to the result's type (half a step)."""
+    x, down, up = s["x"].double(), s["down"].double(), s["up"].double()
+    out, size = s["into"].double().clone(), torch.zeros(s["into"].shape, dtype=torch.float64)
+    rank, k = up.shape[2], x.shape[1]
+    for a in range(down.shape[0]):
+        rows = (s["adapters"] == a).nonzero()[:, 0]
+        inner, inner_size = x[rows] @ down[a].t(), x[rows].abs() @ down[a].abs().t()
+        begin = 0
+        for part, width in enumerate(s["columns"]):
+            mine, factor = slice(part * rank, (part + 1) * rank), up[a, begin: begin + width]
+            out[rows, begin: begin + width] += float(s["scale"][a]) * (inner[:, mine] @ factor.t())
+            size[rows, begin: begin + width] = float(s["scale"][a]) * (inner_size[:, mine] @ factor.abs().t())
+            begin += width
+    half_step = torch.finfo(s["into"].dtype).eps / 2
+    bound = size * ((k + rank + 8) * 2.0 ** -24 + 2.0 ** -17) + out.abs() * (half_step + 2.0 ** -23)
+    return out, bound * (1 + half_step)
+
+
+def run(ops, s, out=None, **views):
+    on = {name: value.cuda() if torch.is_tensor(value) else value for name, value in s.items()}
+    on.update(views)
+    return ops.lora_add(on["x"], on["down"], on["up"], on["scale"], on["adapters"], on["into"], columns=on["columns"], out=out)
+
+
+def check(ops, s):
+    want, bound = definition(s)
+    got = run(ops, s).cpu().double()
+    far = ((got - want).abs() > bound).nonzero()
+    assert len(far) == 0, (len(far), far[:4].tolist(), [(got[tuple(i)].item(), want[tuple(i)].item(), bound[tuple(i)].item()) for i in far[:4]])
+    none = s["adapters"] < 0
+    assert torch.equal(got[none].to(s["into"].dtype), s["into"][none])  # (rows without an adapter: bit by bit)
+
+
+KINDS = [("bfloat16", False), ("bfloat16", True), ("float32", False)]
+
+
+@pytest.mark.parametrize("dtype,stream", KINDS)
+@pytest.mark.parametrize("rows", [1, 2, 15, 16, 17, 33, 64, 65, 130, 300])
+@pytest.mark.parametrize("rank,columns", [(16, (192, 64, 64)), (8, (200,)), (64, (320, 320)), (12, (36, 20))])
+def test_rows_ranks_and_pieces(ops, dtype, stream, rows, rank, columns):
+    check(ops, site(rows, 256, columns, rank, 5, getattr(torch, dtype), stream, seed=rows + rank))
+
+
+@pytest.mark.parametrize("dtype,stream", KINDS)
+@pytest.mark.parametrize("rank", [1, 2, 3, 4, 5, 7, 24, 32, 40, 100, 128])
+def test_ranks(ops, dtype, stream, rank):
+    check(ops, site(37, 136, (80, 48), rank, 3, getattr(torch, dtype), stream, seed=rank))
+
+
+@pytest.mark.parametrize("dtype,stream", KINDS)
+@pytest.mark.parametrize("k", [1, 7, 8, 30, 31, 32, 33, 64, 104, 520, 1000, 4864, 18944])
+def test_lengths_of_a_row(ops, dtype, stream, k):
+    check(ops, site(19, k, (72, 24), 8, 3, getattr(torch, dtype), stream, seed=k))
+
+
+@pytest.mark.parametrize("dtype,stream", KINDS)
+@pytest.mark.parametrize("columns", [(1,), (3, 5), (17, 1, 30), (63, 65, 2, 126), (1000, 24), (15, 16, 17, 18)])
+def test_odd_columns(ops, dtype, stream, columns):
+    for rows in (3, 70):
+        check(ops, site(rows, 96, columns, 16, 4, getattr(torch, dtype), stream, seed=len(columns)))
+
+
+@pytest.mark.parametrize("dtype,stream", KINDS)
+def test_who_has_which_adapter(ops, dtype, stream):
+    """None at all, one for all, every row another one, runs that end inside a tile, numbers that name no adapter."""
+    for seed, adapters in enumerate([
+            [-1] * 70, [2] * 70, [r % 64 for r in range(140)], [r % 3 for r in range(200)], [0] * 63 + [1] * 2 + [3] * 64 + [-1] * 9,
+            [-1] * 40 + [5] + [-1] * 40, [-(1 << 31), -2, 64, (1 << 31) - 1, 1, 63]]):
+        s = site(len(adapters), 104, (48, 32), 16, 64, getattr(torch, dtype), stream, seed=seed, adapters=adapters)
+        check(ops, s)
+        if max(adapters) >= 64:  # (not an adapter: its row stays as it is)
+            got = run(ops, s).cpu()
+            assert torch.equal(got[:4], s["into"][:4])
+
+
+@pytest.mark.parametrize("dtype,stream", KINDS)
+def test_rows_that_lie_apart(ops, dtype, stream):
+    dtype = getattr(torch, dtype)
+    for k, shift in ((128, 8), (128, 1), (100, 3)):
+        s = site(50, k, (96, 40), 16, 3, dtype, stream, seed=k + shift)
+        want, bound = definition(s)
+        x = torch.full((50, k + 24), math.nan, dtype=dtype).cuda()
+        x[:, shift: shift + k] = s["x"].cuda()
+        into = torch.full((50, 136 + 16), 5.0, dtype=s["into"].dtype).cuda()
+        into[:, shift: shift + 136] = s["into"].cuda()
+        out = torch.full((50, 136 + 32), 7.0, dtype=s["into"].dtype).cuda()
+        run(ops, s, out=out[:, shift: shift + 136], x=x[:, shift: shift + k], into=into[:, shift: shift + 136])
+        assert ((out[:, shift: shift + 136].cpu().double() - want).abs() <= bound).all()
+        assert (out[:, :shift] == 7).all() and (out[:, shift + 136:] == 7).all() and (into[:, :shift] == 5).all()
+        run(ops, s, x=x[:, shift: shift + k], into=into[:, shift: shift + 136])  # in place
+        assert torch.equal(into[:, shift: shift + 136], out[:, shift: shift + 136])
+        assert (into[:, :shift] == 5).all() and (into[:, shift + 136:] == 5).all()
+
+
+@pytest.mark.parametrize("dtype,stream", KINDS)
+def test_a_row_depends_on_its_own_adapter_alone(ops, dtype, stream):
+    """Bit by bit the same alone, among others, and beside adapters and rows of infinities and NaN."""
+    s = site(90, 264, (112, 48), 16, 6, getattr(torch, dtype), stream, seed=4)
+    together = run(ops, s).cpu()
+    for r in (0, 1, 17, 64, 89):
+        one = {name: value[r: r + 1] if name in ("x", "adapters", "into") else value for name, value in s.items()}
+        assert torch.equal(run(ops, one).cpu()[0], together[r]), r
+    odd = {name: value.clone() if torch.is_tensor(value) else value for name, value in s.items()}
+    odd["down"][2], odd["up"][2] = math.inf, math.nan
+    odd["x"][s["adapters"] == 2] = math.nan
+    odd["x"][s["adapters"] < 0] = math.inf
+    got = run(ops, odd).cpu()
+    others = s["adapters"] != 2
+    assert torch.equal(got[others], together[others]) and not got[~others].isfinite().any()
+
+
+def test_many_rows_and_columns(ops):
+    """Offsets beyond a tile grid's first dimension, and a prompt whose rows take two adapters."""
+    adapters = [0] * 900 + [2] * 700 + [-1] * 400 + [r % 4 for r in range(48)]
+    check(ops, site(2048, 512, (4864, 4864), 32, 4, torch.bfloat16, seed=2, adapters=adapters))
+    check(ops, site(1100, 3584, (2048,), 8, 3, torch.float32, seed=3))
+
+
+@pytest.mark.parametrize("dtype,stream", KINDS)
+def test_replayed_with_other_adapters(ops, dtype, stream):
+    s = site(21, 256, (128, 64), 16, 4, getattr(torch, dtype), stream, seed=12)
+    on = {name: value.cuda() if torch.is_tensor(value) else value for name, value in s.items()}
+    call = lambda: ops.lora_add(on["x"], on["down"], on["up"], on["scale"], on["adapters"], on["into"],  # noqa: E731
+                                columns=on["columns"], out=torch.empty_like(on["into"]))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):  # (two graphs, whose workspaces must not be one)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, call()))
+        graphs[-1] = (graph, graphs[-1][1])
+    g = torch.Generator().manual_seed(77)
+    for _ in range(3):
+        on["adapters"].copy_(torch.randint(-1, 4, (21,), generator=g).int())
+        on["x"].copy_(torch.randn((21, 256), generator=g))
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        eager = call()
+        assert all(torch.equal(out, eager) for _, out in graphs)
+        now = dict(s, x=on["x"].cpu(), adapters=on["adapters"].cpu())
+        want, bound = definition(now)
+        assert ((eager.cpu().double() - want).abs() <= bound).all()
+
+
+def test_no_rows(ops):
+    s = site(0, 64, (32,), 8, 2, torch.bfloat16)
+    assert run(ops, s).shape == (0, 32)
+
+
+def test_refusals(ops):
+    s = {name: value.cuda() if torch.is_tensor(value) else value for name, value in site(4, 64, (32, 16), 8, 2, torch.bfloat16).items()}
+    ops.lora_add(**s)
+    bad = [
+        dict(x=s["x"].cpu()), dict(x=s["x"].half()), dict(x=s["x"].float()), dict(x=s["x"][:, :63]), dict(x=s["x"][0]),
+        dict(x=s["x"][:1].expand(4, 64)), dict(x=s["x"].t()), dict(down=s["down"][:, :8].contiguous()), dict(down=s["down"][:, :, :32]),
+        dict(down=s["down"][:1]), dict(up=s["up"][:, :, :4].contiguous()), dict(up=s["up"][:, :47].contiguous()), dict(up=s["up"].float()),
+        dict(scale=s["scale"][:1]), dict(scale=s["scale"].double()), dict(adapters=s["adapters"].long()), dict(adapters=s["adapters"][:3]),
+        dict(into=s["into"].half()), dict(into=s["into"][:3]), dict(into=s["into"][:, :47]), dict(columns=(32,)), dict(columns=(32, 17)),
+        dict(columns=(32, 16, 0)), dict(columns=(48, 0)), dict(columns=None), dict(columns=(24, 8, 8, 4, 4)), dict(columns=()),
+        dict(out=s["into"].float()), dict(out=s["into"][:3]), dict(out=s["into"].cpu()),
+    ]
+    for change in bad:
+        with pytest.raises(ValueError):
+            ops.lora_add(**dict(s, **change))
+    wide = site(4, 64, (32,), 129, 2, torch.bfloat16)
+    with pytest.raises(ValueError):
+        run(ops, wide)
+    wide = {name: value.cuda() if torch.is_tensor(value) else value for name, value in site(4, 64, (32,), 8, 2, torch.float32).items()}
+    with pytest.raises(ValueError):
+        ops.lora_add(**dict(wide, into=wide["into"].bfloat16()))
