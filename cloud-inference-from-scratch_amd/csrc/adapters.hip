@@ -4,7 +4,11 @@
 // projections that read the same rows (q, k and v; gate and up): `down` [A, P R, K] has R rows for each, the columns of `out`
 // fall into P pieces, and p(c) is the piece of column c.
 //
-// The sums are float32, the result is rounded once.
+// The sums are float32, the result is rounded once.  Two launches: `down` (K long, few columns; K cut into parts whose float32 sums
+// lie side by side, so that few rows still fill the GPU) and `up` (R long, many columns; it adds the parts in order).  Rows are
+// taken in tiles of consecutive ones; what a tile does is done once for each adapter that its rows have, on these rows alone,
+// gathered into matrix-core tiles of 16.  So no plan of who has which adapter is made on the host, a row's sums do not depend
+// on its neighbours, and a prompt (one adapter) and 64 requests (16 of them) run through the same code.
 #include "common.h"
 
 namespace {
@@ -70,27 +74,688 @@ int run_plain(hipStream_t s, const void* x, long ldx, const void* down, const vo
     return cie_after_launch();
 }
 
+// ---------------------------------------------------------------- tiles
+typedef unsigned long long u64;
+typedef float quad_t __attribute__((ext_vector_type(4)));
+typedef __bf16 octet_t __attribute__((ext_vector_type(8)));
+typedef __bf16 half_octet_t __attribute__((ext_vector_type(4)));
+
+// What a lane hands to a matrix instruction: 16 bytes, `kLane` numbers of one row (lane % 16) that lie together (place
+// lane / 16).  Both operands take their k in the same order, so which k an instruction calls which does not matter.
+template <typename T>
+struct Operand;
+template <>
+struct Operand<bf16_t> {
+    typedef octet_t type;
+    static constexpr int kLane = 8;
+    static __device__ __forceinline__ quad_t mac(type a, type b, quad_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Operand<float> {
+    typedef quad_t type;
+    static constexpr int kLane = 4;
+    static __device__ __forceinline__ quad_t mac(type a, type b, quad_t c) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+        return c;
+    }
+};
+constexpr int kQuarters = 4;  // a wave's lanes hold 4 stretches of kLane k
+constexpr int kWaves = kThreads / kWave;
+constexpr int kTile = 16;
+
+// The rows of a tile that have one adapter, first come first served: lane i learns the i-th of them.
+struct Gathered {
+    int adapter, count, row;
+};
+__device__ __forceinline__ Gathered gather(int id, u64 left) {
+    const int lane = threadIdx.x % kWave;
+    Gathered g;
+    g.adapter = __builtin_amdgcn_readlane(id, __ffsll(left) - 1);
+    const u64 mine = __ballot(id == g.adapter) & left;
+    g.count = __popcll(mine);
+    // (the others go behind them, so that every lane is sent exactly one row)
+    const u64 below = (1ull << lane) - 1;
+    const int place = (mine >> lane) & 1 ? __popcll(mine & below) : g.count + __popcll(~mine & below);
+    g.row = __builtin_amdgcn_ds_permute(place * 4, lane);
+    return g;
+}
+
+// h_part[s, t, j]: the sums of part s of K.  grid: (parts, row tiles, column groups x slots).  A workgroup takes every
+// `slots`-th of its tile's adapters.  K falls into chunks whose length depends on K alone; four waves share a chunk's k and join
+// their sums through LDS, chunks are added one after the other.  A part is one chunk (few rows: as many workgroups as there
+// are) or all of them (many rows: one part): either way h is the same sum in the same order, whatever rows are beside it.
+template <typename T, int C, int R>
+__device__ __forceinline__ void down_rows(const Gathered& g, const T* __restrict__ x, long ldx, const T* __restrict__ down,
+                                          float* __restrict__ part, int row0, int inner, int j0, int k, int k_begin, int k_end,
+                                          int chunk, quad_t (*s_sum)[kWaves][C][kWave]) {
+    typedef Operand<T> Op;
+    constexpr int kStep = Op::kLane * kQuarters, kOwn = (C + kWaves - 1) / kWaves;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, place = lane / kTile * Op::kLane;
+    const T* rows[R];
+    const T* weights[C];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int which = i * kTile + lane % kTile;
+        rows[i] = x + static_cast<size_t>(row0 + __shfl(g.row, which < g.count ? which : 0, kWave)) * ldx;
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int j = j0 + c * kTile + lane % kTile;
+        weights[c] = down + (static_cast<size_t>(g.adapter) * inner + (j < inner ? j : inner - 1)) * k;
+    }
+    quad_t total[R][kOwn], acc[R][C];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+#pragma unroll
+        for (int o = 0; o < kOwn; ++o) total[i][o] = quad_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[i][c] = quad_t{0.f, 0.f, 0.f, 0.f};
+    }
+    // a round is U steps of every wave; the next round is under way while one is multiplied, also across the end of a chunk
+    constexpr int U = R == 1 ? 2 : 1, kRound = kStep * kWaves * U;
+    const int rounds = (k_end - k_begin + kRound - 1) / kRound, rounds_of_chunk = chunk / kRound;
+    typename Op::type a[U][R], b[U][C];
+    const auto ask = [&](int round) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int at = k_begin + (round * U + u) * (kStep * kWaves) + wave * kStep + place;
+            const int from = at < k_end ? at : 0;
+#pragma unroll
+            for (int c = 0; c < C; ++c) b[u][c] = *reinterpret_cast<const typename Op::type*>(weights[c] + from);
+#pragma unroll
+            for (int i = 0; i < R; ++i) a[u][i] = *reinterpret_cast<const typename Op::type*>(rows[i] + from);
+            if (at >= k_end) {  // (k is a multiple of kLane)
+#pragma unroll
+                for (int c = 0; c < C; ++c) b[u][c] = typename Op::type{};
+#pragma unroll
+                for (int i = 0; i < R; ++i) a[u][i] = typename Op::type{};
+            }
+        }
+    };
+    ask(0);
+    int turn = 0;
+    for (int round = 0, of_chunk = 1; round < rounds; ++round, ++of_chunk) {
+        typename Op::type a_now[U][R], b_now[U][C];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int i = 0; i < R; ++i) a_now[u][i] = a[u][i];
+#pragma unroll
+            for (int c = 0; c < C; ++c) b_now[u][c] = b[u][c];
+        }
+        if (round + 1 < rounds) ask(round + 1);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+#pragma unroll
+                for (int c = 0; c < C; ++c) acc[i][c] = Op::mac(a_now[u][i], b_now[u][c], acc[i][c]);
+        if (of_chunk < rounds_of_chunk && round + 1 < rounds) continue;
+        of_chunk = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            // (two buffers in turn: a wave writes one again only behind the barrier of the other)
+            quad_t(*s)[C][kWave] = s_sum[turn];
+            turn ^= 1;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                s[wave][c][lane] = acc[i][c];
+                acc[i][c] = quad_t{0.f, 0.f, 0.f, 0.f};
+            }
+            __syncthreads();
+#pragma unroll
+            for (int o = 0; o < kOwn; ++o) {
+                const int c = wave + o * kWaves;
+                if (c < C) total[i][o] += (s[0][c][lane] + s[1][c][lane]) + (s[2][c][lane] + s[3][c][lane]);
+            }
+        }
+    }
+    __syncthreads();  // (whoever comes next begins with the first buffer)
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int o = 0; o < kOwn; ++o) {
+            const int c = wave + o * kWaves, j = j0 + c * kTile + lane % kTile;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int which = i * kTile + lane / kTile * 4 + e;
+                const int row = __shfl(g.row, which < g.count ? which : 0, kWave);
+                if (c < C && which < g.count && j < inner) part[static_cast<size_t>(row0 + row) * inner + j] = total[i][o][e];
+            }
+        }
+}
+
+template <typename T, int C>
+__global__ void __launch_bounds__(kThreads)
+adapter_down_tiles(const T* __restrict__ x, long ldx, const T* __restrict__ down, const int* __restrict__ adapter,
+                   float* __restrict__ h_part, int rows, int inner, int k, int adapters, int tile_rows, int slots, int chunk,
+                   int part_k) {
+    __shared__ quad_t s_sum[2][kWaves][C][kWave];
+    const int lane = threadIdx.x % kWave, row0 = blockIdx.y * tile_rows;
+    const int slot = blockIdx.z % slots, j0 = blockIdx.z / slots * (C * kTile);
+    int id = lane < tile_rows && row0 + lane < rows ? adapter[row0 + lane] : -1;
+    id = id < adapters ? id : -1;
+    const int k_begin = blockIdx.x * part_k, k_end = min(k, k_begin + part_k);
+    float* part = h_part + static_cast<size_t>(blockIdx.x) * rows * inner;
+    u64 left = __ballot(id >= 0);
+    for (int number = 0; left; ++number) {
+        const Gathered g = gather(id, left);
+        left &= ~__ballot(id == g.adapter);
+        if (number % slots != slot) continue;
+        if (g.count <= kTile)
+            down_rows<T, C, 1>(g, x, ldx, down, part, row0, inner, j0, k, k_begin, k_end, chunk, s_sum);
+        else if (g.count <= 2 * kTile)
+            down_rows<T, C, 2>(g, x, ldx, down, part, row0, inner, j0, k, k_begin, k_end, chunk, s_sum);
+        else
+            down_rows<T, C, 4>(g, x, ldx, down, part, row0, inner, j0, k, k_begin, k_end, chunk, s_sum);
+    }
+}
+
+// The rows of h on their way into the second product.  In bfloat16 a number is two: its rounding and the rounding of what that
+// left out, 16 bits together (2^-17 of the number), so that a float32 stream does not lose the adapter's low bits; the
+// product runs twice, which its 16 to 128 long sums never notice beside the rows they are added to.
+template <typename T>
+struct Inner;
+template <>
+struct Inner<bf16_t> {
+    static constexpr int kHalves = 2;
+    typedef __bf16 store_t;
+    static __device__ __forceinline__ void put(store_t* at, int apart, float v) {
+        const __bf16 high = static_cast<__bf16>(v);
+        const float kept = static_cast<float>(high);
+        at[0] = high;
+        at[apart] = static_cast<__bf16>(fabsf(kept) < INFINITY ? v - kept : 0.f);
+    }
+};
+template <>
+struct Inner<float> {
+    static constexpr int kHalves = 1;
+    typedef float store_t;
+    static __device__ __forceinline__ void put(store_t* at, int, float v) { at[0] = v; }
+};
+
+// kLane numbers of a row of `up` from place k on (rank is a multiple of 4; what lies behind it counts as 0).
+__device__ __forceinline__ octet_t up_numbers(const bf16_t* row, int k, int rank) {
+    if (rank % 8 == 0) return k < rank ? *reinterpret_cast<const octet_t*>(row + k) : octet_t{};
+    half_octet_t lo = {}, hi = {};
+    if (k < rank) lo = *reinterpret_cast<const half_octet_t*>(row + k);
+    if (k + 4 < rank) hi = *reinterpret_cast<const half_octet_t*>(row + k + 4);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ __forceinline__ quad_t up_numbers(const float* row, int k, int rank) {
+    return k < rank ? *reinterpret_cast<const quad_t*>(row + k) : quad_t{};
+}
+
+// 16 bytes of a row of `into`, and what is added to them.
+typedef uint32_t words_t __attribute__((ext_vector_type(4)));
+template <typename S>
+struct Piece {
+    static constexpr int kNumbers = 16 / sizeof(S);
+    static __device__ __forceinline__ words_t sum(words_t old, const float (&more)[kNumbers]);
+};
+template <>
+__device__ __forceinline__ words_t Piece<float>::sum(words_t old, const float (&more)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) old[i] = __float_as_uint(__uint_as_float(old[i]) + more[i]);
+    return old;
+}
+template <>
+__device__ __forceinline__ words_t Piece<bf16_t>::sum(words_t old, const float (&more)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        old[i] = pack_bf16(__uint_as_float(old[i] << 16) + more[2 * i], __uint_as_float(old[i] & 0xffff0000u) + more[2 * i + 1]);
+    return old;
+}
+
+// A wave's share of the second product: the rows of one adapter, 16 at a time, and a strip of columns.  h is the first operand,
+// the strip's columns the second, dealt to the instructions so that a lane's results are 16 bytes of neighbouring columns (in
+// four rows), and 16 lanes have 256 bytes of a row in one piece.
+template <typename T, typename S, int kSteps>
+struct Share {
+    typedef Operand<T> Op;
+    static constexpr int kOwn = Piece<S>::kNumbers, kStrip = kTile * kOwn;
+    typename Op::type weights[kSteps][kOwn];
+    words_t next[4];
+    const int* order;
+    int adapter, count, first;  // first: of the lane's columns
+    bool whole;
+
+    __device__ __forceinline__ void ask_rows(int begin, const S* into, long ld_into) {
+        const int quarter = threadIdx.x % kWave / kTile;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int which = begin + quarter * 4 + i;
+            if (whole && which < count) next[i] = *reinterpret_cast<const words_t*>(into + static_cast<size_t>(order[which]) * ld_into + first);
+        }
+    }
+
+    // (the rows: `count` of them in `order`)
+    __device__ __forceinline__ void ask(const int* order_, int count_, int adapter_, int c0, int end, const T* up, int n, int rank,
+                                        const S* into, long ld_into, bool wide) {
+        const int lane = threadIdx.x % kWave, quarter = lane / kTile;
+        order = order_;
+        count = count_;
+        adapter = adapter_;
+        first = c0 + lane % kTile * kOwn;
+        whole = wide && first + kOwn <= end;
+        if (adapter >= 0) {
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j) {
+                const int c = first + j < end ? first + j : end - 1;
+                const T* from = up + (static_cast<size_t>(adapter) * n + c) * rank;
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s) weights[s][j] = up_numbers(from, (s * kQuarters + quarter) * Op::kLane, rank);
+            }
+        }
+        ask_rows(0, into, ld_into);
+    }
+
+    template <typename H>
+    __device__ __forceinline__ void finish(const H& h, int end, const S* into, long ld_into, S* out, long ld_out) {
+        const int lane = threadIdx.x % kWave, quarter = lane / kTile;
+        for (int begin = 0; begin < count; begin += kTile) {
+            words_t old[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) old[i] = next[i];
+            if (begin + kTile < count) ask_rows(begin + kTile, into, ld_into);
+            quad_t acc[kOwn] = {};
+            if (adapter >= 0) {
+                const int row = order[min(begin + lane % kTile, count - 1)];
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                    for (int half = 0; half < Inner<T>::kHalves; ++half) {
+                        const typename Op::type mine =
+                            *reinterpret_cast<const typename Op::type*>(&h[half][row][(s * kQuarters + quarter) * Op::kLane]);
+#pragma unroll
+                        for (int j = 0; j < kOwn; ++j) acc[j] = Op::mac(mine, weights[s][j], acc[j]);
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int which = begin + quarter * 4 + i;
+                if (which >= count) continue;
+                const int row = order[which];
+                S* to = out + static_cast<size_t>(row) * ld_out + first;
+                if (whole) {
+                    float more[kOwn];
+#pragma unroll
+                    for (int j = 0; j < kOwn; ++j) more[j] = acc[j][i];
+                    *reinterpret_cast<words_t*>(to) = adapter >= 0 ? Piece<S>::sum(old[i], more) : old[i];
+                    continue;
+                }
+                const S* from = into + static_cast<size_t>(row) * ld_into + first;
+#pragma unroll
+                for (int j = 0; j < kOwn; ++j)
+                    if (first + j < end) to[j] = adapter >= 0 ? from_float<S>(to_float(from[j]) + acc[j][i]) : from[j];
+            }
+        }
+    }
+};
+
+// Who of a row tile has which adapter.
+struct Order {
+    int id[kWave], order[kWave];  // the rows' adapters (-1: none, or not this workgroup's); the rows by adapter,
+    int group[kWave + 1], count;  // where each adapter's rows begin, and how many adapters there are
+
+    // Every `slots`-th of the adapters that the rows have; rows without one count as one more where they are to be copied.
+    __device__ __forceinline__ void sort_rows(const int* adapter, int row0, int rows, int adapters, int slots, int slot, bool copies) {
+        const int lane = threadIdx.x % kWave;
+        if (threadIdx.x < kWave) {
+            int mine = row0 + lane < rows ? adapter[row0 + lane] : -1;
+            mine = mine >= 0 && mine < adapters ? mine : -1;
+            u64 left = __ballot(row0 + lane < rows && (mine >= 0 || copies));
+            int groups = 0, taken = 0;
+            bool own = false;
+            for (int number = 0; left; ++number) {
+                const u64 same = __ballot(mine == __builtin_amdgcn_readlane(mine, __ffsll(left) - 1)) & left;
+                left &= ~same;
+                if (number % slots != slot) continue;
+                if ((same >> lane) & 1) {
+                    own = true;
+                    order[taken + __popcll(same & ((1ull << lane) - 1))] = lane;
+                }
+                if (lane == 0) group[groups] = taken;
+                ++groups;
+                taken += __popcll(same);
+            }
+            if (lane == 0) {
+                group[groups] = taken;
+                count = groups;
+            }
+            id[lane] = own ? mine : -1;
+        }
+        __syncthreads();
+    }
+};
+
+// ... and its rows of h: the parts added in order, times the adapter's scale.
+template <typename T, int kSteps>
+struct Rows {
+    typedef typename Inner<T>::store_t store_t;
+    static constexpr int kWidth = kSteps * Operand<T>::kLane * kQuarters, kHalves = Inner<T>::kHalves;
+    static constexpr int kLd = kWidth + 16 / sizeof(store_t);  // (rows a little apart, so that 16 of them do not share their banks)
+    store_t number[kHalves][kWave][kLd];
+
+    __device__ __forceinline__ void add_parts(const Order& tile, const float* h_part, int parts, const float* scale, int row0, int rows,
+                                              int inner, int from, int rank) {
+        constexpr int kFours = kWidth / 4;
+        for (int item = threadIdx.x; item < kWave * kFours; item += kThreads) {
+            const int row = item / kFours, r = item % kFours * 4, a = tile.id[row];
+            if (a < 0) continue;
+            quad_t sum = {0.f, 0.f, 0.f, 0.f};
+            if (r < rank) {
+                const float* at = h_part + static_cast<size_t>(row0 + row) * inner + from + r;
+#pragma unroll 8
+                for (int s = 0; s < parts; ++s) sum += *reinterpret_cast<const quad_t*>(at + static_cast<size_t>(s) * rows * inner);
+                sum *= scale[a];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) Inner<T>::put(&number[0][row][r + e], kWave * kLd, sum[e]);
+        }
+        __syncthreads();
+    }
+};
+
+// Which piece, and which of its columns, the block of that number has.
+struct Columns {
+    int piece, begin, end;
+    __device__ __forceinline__ Columns(const Pieces& pieces, int number, int block) {
+        piece = 0;
+        for (; piece + 1 < pieces.count; ++piece) {
+            const int blocks = (pieces.begin[piece + 1] - pieces.begin[piece] + block - 1) / block;
+            if (number < blocks) break;
+            number -= blocks;
+        }
+        begin = pieces.begin[piece] + number * block;
+        end = min(pieces.begin[piece + 1], begin + block);
+    }
+};
+
+// Few rows.  grid: (row tiles, column blocks of the pieces, slots): a workgroup takes every `slots`-th of its tile's adapters, a
+// wave one of them and a strip of columns at a time.  A wave's first weights and rows of `into` are under way while the parts of h
+// are added.
+template <typename T, typename S, int kSteps>
+__global__ void __launch_bounds__(kThreads)
+adapter_up_rows(const float* __restrict__ h_part, int parts, const T* __restrict__ up, const float* __restrict__ scale,
+                const int* __restrict__ adapter, const S* into, long ld_into, S* out, long ld_out, int rows, int inner, int n, int rank,
+                int adapters, Pieces pieces, int block, int slots, bool wide) {
+    __shared__ Order tile;
+    __shared__ __align__(16) Rows<T, kSteps> h;
+    const int wave = threadIdx.x / kWave, row0 = blockIdx.x * kWave;
+    const Columns columns(pieces, blockIdx.y, block);
+    tile.sort_rows(adapter, row0, rows, adapters, slots, blockIdx.z, static_cast<const void*>(into) != static_cast<const void*>(out));
+    if (tile.count == 0) return;
+    into += static_cast<size_t>(row0) * ld_into;
+    out += static_cast<size_t>(row0) * ld_out;
+    constexpr int kStrip = Share<T, S, kSteps>::kStrip;
+    const int strips = (columns.end - columns.begin + kStrip - 1) / kStrip, shares = tile.count * strips;
+    Share<T, S, kSteps> share;
+    const auto ask = [&](int number) {
+        const int group = number / strips, from = tile.group[group];
+        share.ask(tile.order + from, tile.group[group + 1] - from, tile.id[tile.order[from]], columns.begin + number % strips * kStrip,
+                  columns.end, up, n, rank, into, ld_into, wide);
+    };
+    int number = wave;
+    if (number < shares) ask(number);
+    h.add_parts(tile, h_part, parts, scale, row0, rows, inner, columns.piece * rank, rank);
+    while (number < shares) {
+        share.finish(h.number, columns.end, into, ld_into, out, ld_out);
+        number += kWaves;
+        if (number < shares) ask(number);
+    }
+}
+
+// Many rows.  grid: (row tiles, column blocks of the pieces).  A workgroup goes through its strips of columns, and in each through
+// its tile's adapters (of a prompt there is one); each of its four waves has 16 of the adapter's rows, whose h it keeps in
+// registers.  The strip's weights pass through LDS, which all four read, a strip ahead of its use.
+template <typename T, typename S, int kSteps>
+__global__ void __launch_bounds__(kThreads, 4)
+adapter_up_strips(const float* __restrict__ h_part, int parts, const T* __restrict__ up, const float* __restrict__ scale,
+                  const int* __restrict__ adapter, const S* into, long ld_into, S* out, long ld_out, int rows, int inner, int n, int rank,
+                  int adapters, Pieces pieces, int block, bool wide) {
+    typedef Operand<T> Op;
+    typedef typename Inner<T>::store_t store_t;
+    constexpr int kOwn = Piece<S>::kNumbers, kStrip = kTile * kOwn, kLoads = kSteps * kQuarters, kMine = kStrip * kLoads / kThreads;
+    typedef Rows<T, kSteps> RowsT;
+    constexpr int kLd = RowsT::kLd, kHalves = RowsT::kHalves;
+    static_assert(kStrip * kLoads % kThreads == 0, "every thread stages as many pieces");
+    __shared__ Order tile;
+    // Two buffers of weights in turn.  A tile of several adapters has them one after the other in the first, with a barrier more,
+    // and its rows of h in place of the second.
+    struct Weights {
+        store_t number[kStrip][kLd];
+    };
+    constexpr size_t kSecond = sizeof(Weights) > sizeof(RowsT) ? sizeof(Weights) : sizeof(RowsT);
+    __shared__ __align__(16) char lds[sizeof(Weights) + kSecond];
+    Weights* const s_w = reinterpret_cast<Weights*>(lds);
+    RowsT& s_h = *reinterpret_cast<RowsT*>(lds + sizeof(Weights));
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, quarter = lane / kTile, row0 = blockIdx.x * kWave;
+    const Columns columns(pieces, blockIdx.y, block);
+    tile.sort_rows(adapter, row0, rows, adapters, 1, 0, static_cast<const void*>(into) != static_cast<const void*>(out));
+    if (tile.count == 0) return;
+    into += static_cast<size_t>(row0) * ld_into;
+    out += static_cast<size_t>(row0) * ld_out;
+    const int groups = tile.count, total = (columns.end - columns.begin + kStrip - 1) / kStrip * groups;
+
+    typename Op::type staged[kMine], h[kHalves][kSteps];
+    words_t old[4];
+    const auto ask_weights = [&](int number) {
+        const int a = tile.id[tile.order[tile.group[number % groups]]];
+        if (a < 0) return;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int item = i * kThreads + threadIdx.x, c = min(columns.begin + number / groups * kStrip + item / kLoads, columns.end - 1);
+            staged[i] = up_numbers(up + (static_cast<size_t>(a) * n + c) * rank, item % kLoads * Op::kLane, rank);
+        }
+    };
+    // (column c lies where the lane that computes it reads without sharing banks)
+    const auto put_weights = [&](int number) {  // (of the buffer)
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int item = i * kThreads + threadIdx.x, c = item / kLoads;
+            *reinterpret_cast<typename Op::type*>(&s_w[number].number[c % kOwn * kTile + c / kOwn][item % kLoads * Op::kLane]) = staged[i];
+        }
+    };
+    const auto ask_rows = [&](int number) {
+        const int from = tile.group[number % groups], count = tile.group[number % groups + 1] - from;
+        const int first = columns.begin + number / groups * kStrip + lane % kTile * kOwn;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int which = wave * kTile + quarter * 4 + i;
+            if (wide && first + kOwn <= columns.end && which < count)
+                old[i] = *reinterpret_cast<const words_t*>(into + static_cast<size_t>(tile.order[from + which]) * ld_into + first);
+        }
+    };
+    const bool many = groups > 1;
+    const auto ask_h = [&]() {  // of a tile's one adapter
+        const int row = tile.order[min(wave * kTile + lane % kTile, tile.group[1] - 1)], a = tile.id[row];
+        if (a < 0) return;
+        const float factor = scale[a];
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int r = (s * kQuarters + quarter) * Op::kLane;
+            const float* at = h_part + static_cast<size_t>(row0 + row) * inner + columns.piece * rank + r;
+            store_t both[kHalves][Op::kLane];
+#pragma unroll
+            for (int e = 0; e < Op::kLane; e += 4) {
+                quad_t sum = {0.f, 0.f, 0.f, 0.f};
+                if (r + e < rank) {
+                    for (int p = 0; p < parts; ++p) sum += *reinterpret_cast<const quad_t*>(at + e + static_cast<size_t>(p) * rows * inner);
+                    sum *= factor;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) Inner<T>::put(&both[0][e + i], Op::kLane, sum[i]);
+            }
+#pragma unroll
+            for (int half = 0; half < kHalves; ++half)
+#pragma unroll
+                for (int e = 0; e < Op::kLane; ++e) h[half][s][e] = both[half][e];
+        }
+    };
+    ask_weights(0);
+    ask_rows(0);
+    if (many)
+        s_h.add_parts(tile, h_part, parts, scale, row0, rows, inner, columns.piece * rank, rank);
+    else
+        ask_h();
+    for (int number = 0; number < total; ++number) {
+        if (many) __syncthreads();  // (the buffer has been read by all)
+        const int buffer = many ? 0 : number & 1;
+        put_weights(buffer);
+        __syncthreads();  // (and the other buffer has been read by all)
+        if (number + 1 < total) ask_weights(number + 1);
+        const int from = tile.group[number % groups], count = tile.group[number % groups + 1] - from, a = tile.id[tile.order[from]];
+        const int first = columns.begin + number / groups * kStrip + lane % kTile * kOwn;
+        const bool whole = wide && first + kOwn <= columns.end;
+        quad_t acc[kOwn] = {};
+        if (a >= 0 && wave * kTile < count) {
+            if (many) {
+                const int row = tile.order[from + min(wave * kTile + lane % kTile, count - 1)];
+#pragma unroll
+                for (int half = 0; half < kHalves; ++half)
+#pragma unroll
+                    for (int s = 0; s < kSteps; ++s)
+                        h[half][s] = *reinterpret_cast<const typename Op::type*>(&s_h.number[half][row][(s * kQuarters + quarter) * Op::kLane]);
+            }
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                for (int j = 0; j < kOwn; ++j) {
+                    const typename Op::type weights =
+                        *reinterpret_cast<const typename Op::type*>(&s_w[buffer].number[j * kTile + lane % kTile][(s * kQuarters + quarter) * Op::kLane]);
+#pragma unroll
+                    for (int half = 0; half < kHalves; ++half) acc[j] = Op::mac(h[half][s], weights, acc[j]);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int which = wave * kTile + quarter * 4 + i;
+            if (which >= count) continue;
+            const int row = tile.order[from + which];
+            S* to = out + static_cast<size_t>(row) * ld_out + first;
+            if (whole) {
+                float more[kOwn];
+#pragma unroll
+                for (int j = 0; j < kOwn; ++j) more[j] = acc[j][i];
+                *reinterpret_cast<words_t*>(to) = a >= 0 ? Piece<S>::sum(old[i], more) : old[i];
+                continue;
+            }
+            const S* source = into + static_cast<size_t>(row) * ld_into + first;
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j)
+                if (first + j < columns.end) to[j] = a >= 0 ? from_float<S>(to_float(source[j]) + acc[j][i]) : source[j];
+        }
+        if (number + 1 < total) ask_rows(number + 1);
+    }
+}
+
+struct Plan {
+    int chunk, parts, tile_rows, slots, block, up_slots;
+};
+
+template <typename T, int C>
+int launch_down(hipStream_t s, const T* x, long ldx, const T* down, const int* adapter, float* h, int rows, int k, int inner, int adapters,
+                const Plan& plan) {
+    const int part_k = plan.parts == 1 ? (k + plan.chunk - 1) / plan.chunk * plan.chunk : plan.chunk;
+    const int groups = (inner + C * kTile - 1) / (C * kTile);
+    const dim3 grid(plan.parts, (rows + plan.tile_rows - 1) / plan.tile_rows, groups * plan.slots);
+    adapter_down_tiles<T, C><<<grid, kThreads, 0, s>>>(x, ldx, down, adapter, h, rows, inner, k, adapters, plan.tile_rows, plan.slots,
+                                                       plan.chunk, part_k);
+    return cie_after_launch();
+}
+
+template <typename T, typename S>
+int run_tiles(hipStream_t s, const void* x_, long ldx, const void* down_, const void* up_, const float* scale, const int* adapter,
+              const void* into_, long ld_into, void* out_, long ld_out, float* h, int rows, int k, int n, int rank, int adapters,
+              const Pieces& pieces, const Plan& plan) {
+    const T *x = static_cast<const T*>(x_), *down = static_cast<const T*>(down_), *up = static_cast<const T*>(up_);
+    const S* into = static_cast<const S*>(into_);
+    S* out = static_cast<S*>(out_);
+    const int inner = pieces.count * rank;
+    int code = inner <= kTile ? launch_down<T, 1>(s, x, ldx, down, adapter, h, rows, k, inner, adapters, plan)
+               : inner <= 2 * kTile ? launch_down<T, 2>(s, x, ldx, down, adapter, h, rows, k, inner, adapters, plan)
+                                    : launch_down<T, 4>(s, x, ldx, down, adapter, h, rows, k, inner, adapters, plan);
+    if (code != CIE_OK) return code;
+    int blocks = 0;
+    bool wide = ld_into * sizeof(S) % 16 == 0 && ld_out * sizeof(S) % 16 == 0 && reinterpret_cast<uintptr_t>(into) % 16 == 0 &&
+                reinterpret_cast<uintptr_t>(out) % 16 == 0;
+    for (int p = 0; p < pieces.count; ++p) {
+        blocks += (pieces.begin[p + 1] - pieces.begin[p] + plan.block - 1) / plan.block;
+        wide = wide && pieces.begin[p] * sizeof(S) % 16 == 0;
+    }
+    const unsigned row_tiles = (rows + kWave - 1) / kWave;
+    constexpr int kStep = Operand<T>::kLane * kQuarters;
+    if (plan.up_slots > 0) {
+#define CIE_UP(STEPS)                                                                                                              \
+    adapter_up_rows<T, S, STEPS><<<dim3(row_tiles, blocks, plan.up_slots), kThreads, 0, s>>>(                                          \
+        h, plan.parts, up, scale, adapter, into, ld_into, out, ld_out, rows, inner, n, rank, adapters, pieces, plan.block, plan.up_slots, wide)
+        if (rank <= kStep)
+            CIE_UP(1);
+        else if (rank <= 2 * kStep)
+            CIE_UP(2);
+        else if (rank <= 4 * kStep)
+            CIE_UP(4);
+        else if constexpr (kStep * 4 < 128)
+            CIE_UP(8);
+#undef CIE_UP
+    } else {
+#define CIE_UP(STEPS)                                                                                                        \
+    adapter_up_strips<T, S, STEPS><<<dim3(row_tiles, blocks), kThreads, 0, s>>>(h, plan.parts, up, scale, adapter, into, ld_into, out, \
+                                                                              ld_out, rows, inner, n, rank, adapters, pieces, plan.block, wide)
+        if (rank <= kStep)
+            CIE_UP(1);
+        else if (rank <= 2 * kStep)
+            CIE_UP(2);
+        else if constexpr (kStep * 2 < 64)
+            CIE_UP(4);
+#undef CIE_UP
+    }
+    return cie_after_launch();
+}
+
 }  // namespace
 
 // dtype: of x, down and up; out_dtype: of into and out (dtype, or float32).  c1, c2, c3: where the second and later pieces begin
-// (n where there is none).  h: rows * pieces * rank floats.  out may be into.
+// (n where there is none).  out may be into.  parts = 0: the kernels that take any shape (h: rows * pieces * rank floats).  Else the
+// tiles, which take a rank that is a multiple of 4 and rows of x and down in 16-byte pieces: K in chunks of `chunk`, each of them
+// a part or all of them one (h: as many floats for each part), `down` in tiles of tile_rows (16 to 64) rows and `slots` workgroups
+// for a tile's adapters, `up` in blocks of `block` columns; up_slots > 0: in the form for few
+// rows, with so many workgroups for the adapters of a tile of 64 rows, 0: in the form for many (a rank of up to 64).
 CIE_API int cie_lora_add(void* stream, int dtype, int out_dtype, const void* x, long ldx, const void* down, const void* up,
                          const float* scale, const int* adapter, const void* into, long ld_into, void* out, long ld_out, float* h,
-                         int rows, int k, int n, int rank, int adapters, int piece_count, int c1, int c2, int c3) {
-    if (rows < 0 || rows > 65535 || k <= 0 || n <= 0 || rank <= 0 || adapters <= 0 || piece_count < 1 || piece_count > kMaxPieces ||
-        ldx < k || ld_into < n || ld_out < n || !x || !down || !up || !scale || !adapter || !into || !out || !h)
+                         int rows, int k, int n, int rank, int adapters, int piece_count, int c1, int c2, int c3, int chunk,
+                         int parts, int tile_rows, int slots, int block, int up_slots) {
+    if (rows < 0 || rows > 65535 || k <= 0 || n <= 0 || rank <= 0 || rank > 128 || adapters <= 0 || piece_count < 1 ||
+        piece_count > kMaxPieces || ldx < k || ld_into < n || ld_out < n || !x || !down || !up || !scale || !adapter || !into || !out || !h)
         return CIE_BAD_ARGUMENT;
     if (rows == 0) return CIE_OK;
     Pieces pieces = {piece_count, {0, c1, c2, c3, n}};
     for (int p = piece_count; p <= kMaxPieces; ++p) pieces.begin[p] = n;
     for (int p = 0; p < piece_count; ++p)
         if (pieces.begin[p + 1] <= pieces.begin[p]) return CIE_BAD_ARGUMENT;
+    const Plan plan = {chunk, parts, tile_rows, slots, block, up_slots};
+    if (parts != 0) {
+        const int size = dtype == CIE_BF16 ? 2 : 4;
+        const bool lines = k * size % 16 == 0 && ldx * size % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
+                           reinterpret_cast<uintptr_t>(down) % 16 == 0 && reinterpret_cast<uintptr_t>(up) % 16 == 0 &&
+                           reinterpret_cast<uintptr_t>(h) % 16 == 0;
+        const int share = 256 / size;  // (the k that a workgroup's four waves take at a time)
+        if (!lines || rank % 4 || chunk < 2 * share || chunk % (2 * share) || (parts != 1 && parts != (k + chunk - 1) / chunk) || tile_rows < 16 ||
+            tile_rows > kWave || tile_rows % kTile || slots < 1 || slots > kWave || block < kWave || block % kWave || up_slots < 0 ||
+            up_slots > kWave || (up_slots == 0 && rank > 64))
+            return CIE_BAD_ARGUMENT;
+    }
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (dtype == CIE_F32 && out_dtype == CIE_F32)
-        return run_plain<float, float>(s, x, ldx, down, up, scale, adapter, into, ld_into, out, ld_out, h, rows, k, n, rank, adapters, pieces);
-    if (dtype == CIE_BF16 && out_dtype == CIE_F32)
-        return run_plain<bf16_t, float>(s, x, ldx, down, up, scale, adapter, into, ld_into, out, ld_out, h, rows, k, n, rank, adapters, pieces);
-    if (dtype == CIE_BF16 && out_dtype == CIE_BF16)
-        return run_plain<bf16_t, bf16_t>(s, x, ldx, down, up, scale, adapter, into, ld_into, out, ld_out, h, rows, k, n, rank, adapters, pieces);
+#define CIE_RUN(T, S)                                                                                                              \
+    return parts == 0 ? run_plain<T, S>(s, x, ldx, down, up, scale, adapter, into, ld_into, out, ld_out, h, rows, k, n, rank, adapters,  \
+                                        pieces)                                                                                     \
+                      : run_tiles<T, S>(s, x, ldx, down, up, scale, adapter, into, ld_into, out, ld_out, h, rows, k, n, rank, adapters,  \
+                                        pieces, plan)
+    if (dtype == CIE_F32 && out_dtype == CIE_F32) CIE_RUN(float, float);
+    if (dtype == CIE_BF16 && out_dtype == CIE_F32) CIE_RUN(bf16_t, float);
+    if (dtype == CIE_BF16 && out_dtype == CIE_BF16) CIE_RUN(bf16_t, bf16_t);
+#undef CIE_RUN
     return CIE_BAD_ARGUMENT;
 }

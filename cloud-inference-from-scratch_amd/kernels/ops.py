@@ -1552,6 +1552,22 @@ MAX_ADAPTER_RANK = 128
 MAX_ADAPTER_PIECES = 4
 
 
+@functools.lru_cache(maxsize=4096)
+def plan_lora(rows: int, k: int, n: int, inner: int, rank: int, count: int, share: int, units: int) -> tuple[int, int, int, int, int, int]:
+    """(k of a chunk, parts, rows of a tile of the first product, workgroups for a tile's adapters, columns of a workgroup of the
+    second product, workgroups for the adapters of its 64 rows) of :func:`lora_add`.  ``share``: the k that a workgroup takes at
+    a time.  The chunk goes by K alone, so that the sums do."""
+    chunk = max(1, -(-k // (32 * share))) * 2 * share
+    few = rows * inner * -(-k // chunk) <= 1 << 20
+    tile_rows = 64 if rows <= 128 else 16
+    slots = min(count, rows, 16 if rows <= 128 else 2)
+    parts = -(-k // chunk) if few else 1
+    tiles, strips = -(-rows // 64), -(-n // 128)
+    up_slots = 0 if rows > 128 and rank <= 64 else min(count, rows, 8)
+    block = 128 * max(1, -(-strips * tiles // (4 * units)))
+    return chunk, parts, tile_rows, slots, block, up_slots
+
+
 def lora_add(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale: torch.Tensor, adapters: torch.Tensor,
              into: torch.Tensor, columns: Optional[tuple] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``out[t] = into[t] + scale[a] * up[a] @ (down[a] @ x[t])`` with ``a = adapters[t]``: every row's own low-rank adapter beside
@@ -1590,12 +1606,18 @@ def lora_add(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale: torch
         raise ValueError(f"up to 65,535 rows, not {rows}")
     if rows == 0:
         return out
-    inner = torch.empty(rows * pieces * rank, dtype=torch.float32, device=x.device)
+    size = x.element_size()
+    if (rank % 4 == 0 and k * size % 16 == 0 and _ld(x) * size % 16 == 0 and x.data_ptr() % 16 == 0 and down.data_ptr() % 16 == 0
+            and up.data_ptr() % 16 == 0):
+        plan = plan_lora(rows, k, n, pieces * rank, rank, count, 256 // size, compute_units())
+    else:  # (a rank or a row that 16-byte loads do not take)
+        plan = (0, 0, 0, 0, 0, 0)
+    inner = torch.empty(max(1, plan[1]) * rows * pieces * rank, dtype=torch.float32, device=x.device)
     begins = [sum(columns[:p]) for p in range(1, pieces)] + [n] * (MAX_ADAPTER_PIECES - pieces)
     _run("cie_lora_add", load_library().cie_lora_add(
         _stream(), _i(code), _i(_code(into.dtype)), _ptr(x), _i(_ld(x)), _ptr(down), _ptr(up), _ptr(scale), _ptr(adapters),
         _ptr(into), _i(_ld(into)), _ptr(out), _i(_ld(out)), _ptr(inner), _i(rows), _i(k), _i(n), _i(rank), _i(count), _i(pieces),
-        _i(begins[0]), _i(begins[1]), _i(begins[2])))
+        _i(begins[0]), _i(begins[1]), _i(begins[2]), *plan))
     return out
 
 
