@@ -1504,15 +1504,16 @@ def _per_row(name: str, t: torch.Tensor, dtype: torch.dtype, rows: int) -> None:
         raise ValueError(f"{name} must be [{rows}], is {list(t.shape)}")
 
 
-MAX_RULE_ROWS = 65535
+MAX_RULE_ROWS, MAX_RULE_VOCAB = 65535, 1 << 24
+RULES_PART = 4096  # logits of a part of the first launch, whose results take 130 words of 8 bytes
 
 
 def _sample_rules(logits, temperature, uniform, out, top_k, top_p, min_p) -> torch.Tensor:
     rows, vocab = _logit_rows(logits)
     if temperature is None or uniform is None:
         raise ValueError("a draw under rules needs temperatures and uniform numbers")
-    if rows > MAX_RULE_ROWS:
-        raise ValueError(f"up to {MAX_RULE_ROWS} rows, not {rows}")
+    if rows > MAX_RULE_ROWS or vocab > MAX_RULE_VOCAB:
+        raise ValueError(f"up to {MAX_RULE_ROWS} rows of {MAX_RULE_VOCAB} logits, not {rows} of {vocab}")
     _per_row("temperature", temperature, torch.float32, rows)
     _per_row("uniform", uniform, torch.float32, rows)
     for name, rule, dtype in (("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
@@ -1524,9 +1525,10 @@ def _sample_rules(logits, temperature, uniform, out, top_k, top_p, min_p) -> tor
     _on_current_gpu(logits, temperature, uniform, top_k, top_p, min_p, out)
     if rows == 0:
         return out
+    work = torch.empty(rows * -(-vocab // RULES_PART) * 130, dtype=torch.int64, device=logits.device)
     _run("cie_sample_rules", load_library().cie_sample_rules(
-        _stream(), _ptr(logits), _ptr(temperature), _ptr(uniform), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(out), _i(rows),
-        _i(vocab), _i(_ld(logits))))
+        _stream(), _ptr(logits), _ptr(temperature), _ptr(uniform), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(out), _ptr(work),
+        _i(rows), _i(vocab), _i(_ld(logits))))
     return out
 
 
