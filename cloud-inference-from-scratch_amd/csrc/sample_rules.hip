@@ -10,14 +10,16 @@
 //   (A token of less than 2^-45 of the largest weight, for 152,000 tokens, is not drawn: see below.)
 // A row in which nothing weighs anything gives index 0.
 //
-// Two launches.  The first reads the logits once, in parts that fill the GPU: the largest of each part, of each 16 numbers (a
-// chunk), and, for rows that draw from all tokens or from a share of all weight, the part's sum of weights.  The second has a
-// workgroup for each row, which with that rarely needs the row again: the k-th largest of the chunks' largest is a bound
-// that the k largest logits reach, a share p of the weight cannot reach down to tokens that weigh less than (1 - p) / vocab of
-// the sum, min-p names its bound itself.  It gathers what passes the bound from the few chunks whose largest does, sorts it, and
-// cuts and draws in LDS.  Where more than kList numbers pass (flat rows), the row is walked: a histogram of its weights, then
-// the numbers of the one bin that holds the cut.  Rows that defeat that too (thousands of equal logits at the cut) are cut by the
-// bits of their logits.
+// The first launch reads the logits once, in parts that fill the GPU: the largest of each part, of each 16 numbers (a chunk), and,
+// for rows without top-k, the part's sum of weights.  The last has a workgroup for each row.
+//   top-k: the k-th largest of the chunks' largest is a bound that the k largest logits reach; what passes it, from the few
+//     chunks whose largest does, is gathered, ranked, cut and drawn from in LDS.
+//   top-p or min-p without top-k: a share p of the weight cannot reach down to tokens that weigh less than (1 - p) / vocab of
+//     the sum, and min-p names its bound itself.  Two launches between the others go through the chunks that pass the bound: one adds
+//     the weights to the row's histogram over equal bins of (max - l) / T, the other finds the bin that holds the cut, sums the
+//     weights in front of it part by part and lists the bin's numbers.  The last one sorts these, and walks the part it draws from.
+//   no rule: the parts' sums say which part is walked.
+// Rows that defeat this (more than kList logits that pass a k's bound, or in the cut's bin) are cut by the bits of their logits.
 //
 // Every rule keeps a prefix of one order, so what is kept is said by one cut: a logit, and of the tokens that are equal to it
 // the last index.
@@ -276,17 +278,41 @@ __device__ int draw_by_bits(Row& row, Histogram& h, u64* s_sum, int k, double p,
 constexpr int kPartThreads = 256;
 constexpr int kPart = kPartThreads * 16;  // numbers of a part: a thread has four times four neighbours, 1,024 numbers apart
 
+constexpr int kList = 4096;
+constexpr int kMaxParts = 2048;
+
 struct PartOf {
     u64* best;       // [rows, parts] order << 32 | (0x7fffffff - index) of the largest
     double* sum;     // [rows, parts] sum of exp((l - the part's largest) / T), where the row asks for it
     float* chunk;    // [rows, parts * kPartThreads] the largest of each thread's 16; -inf where there is none
+    // of rows under top-p or min-p without top-k:
+    u64* kept;       // [rows, parts] weight of what lies in front of the cut's bin
+    u64* histogram;  // [rows, kBins]
+    u64* list;       // [rows, kList] the numbers of the cut's bin
+    u64* head;       // [rows, 2] how many these are; what lies in front of them
 };
 
-__device__ __forceinline__ bool wants_sum(float temp, int k, int vocab) { return temp > 0.f && !(k > 0 && k < vocab); }
+__device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+
+// The rules of a row as they count: k = 0, p = 1 and m = 0 are off (NaN too).
+struct Rules {
+    float temp;
+    int k;
+    double p, m;
+    __device__ __forceinline__ Rules(const float* temperature, const int* top_k, const float* top_p, const float* min_p, int r, int vocab) {
+        temp = temperature[r];
+        k = top_k && top_k[r] > 0 && top_k[r] < vocab ? top_k[r] : 0;
+        p = top_p && top_p[r] < 1.f ? (top_p[r] > 0.f ? static_cast<double>(top_p[r]) : 0.0) : 1.0;
+        m = min_p && min_p[r] > 0.f ? (min_p[r] < 1.f ? static_cast<double>(min_p[r]) : 1.0) : 0.0;  // (the largest stays)
+    }
+    __device__ __forceinline__ bool draws() const { return temp > 0.f; }
+    __device__ __forceinline__ bool shares() const { return temp > 0.f && k == 0; }          // needs the parts' sums
+    __device__ __forceinline__ bool tallied() const { return shares() && (p < 1.0 || m > 0.0); }
+};
 
 __global__ void __launch_bounds__(kPartThreads)
-rules_parts_kernel(const float* __restrict__ logits, const float* __restrict__ temperature, const int* __restrict__ top_k, PartOf of,
-                   int vocab, long ld) {
+rules_parts_kernel(const float* __restrict__ logits, const float* __restrict__ temperature, const int* __restrict__ top_k,
+                   const float* __restrict__ top_p, const float* __restrict__ min_p, PartOf of, int vocab, long ld) {
     constexpr int kPartWaves = kPartThreads / kWave;
     __shared__ u64 s_best[kPartWaves];
     __shared__ double s_sum[kPartWaves];
@@ -321,7 +347,7 @@ rules_parts_kernel(const float* __restrict__ logits, const float* __restrict__ t
     }
     u64 best = (static_cast<u64>(key) << 32) | static_cast<uint32_t>(0x7fffffff - where);
     // the order's float (a chunk of NaN alone counts as -inf)
-    const float largest = key <= kOrderOfMinusInf ? -INFINITY : __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+    const float largest = key <= kOrderOfMinusInf ? -INFINITY : logit_of(key);
     of.chunk[(static_cast<size_t>(r) * gridDim.x + part) * kPartThreads + threadIdx.x] = largest;
 #pragma unroll
     for (int offset = kWave / 2; offset > 0; offset >>= 1) {
@@ -333,12 +359,16 @@ rules_parts_kernel(const float* __restrict__ logits, const float* __restrict__ t
 #pragma unroll
     for (int w = 0; w < kPartWaves; ++w) best = s_best[w] > best ? s_best[w] : best;
     if (threadIdx.x == 0) of.best[static_cast<size_t>(r) * gridDim.x + part] = best;
-    const float temp = temperature[r];
-    if (!wants_sum(temp, top_k ? top_k[r] : 0, vocab)) return;
+    const Rules rules(temperature, top_k, top_p, min_p, r, vocab);
+    if (!rules.shares()) return;
+    if (rules.tallied()) {  // (the launches behind this one add to them)
+        for (int b = part * kPartThreads + threadIdx.x; b < kBins; b += gridDim.x * kPartThreads) of.histogram[static_cast<size_t>(r) * kBins + b] = 0;
+        if (part == 0 && threadIdx.x == 0) of.head[2 * r] = 0;
+    }
     key = static_cast<uint32_t>(best >> 32);
     double sum = 0.0;
     if (key > kOrderOfMinusInf) {
-        const Row scaled = {row, vocab, __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key), 1.0 / static_cast<double>(temp), 1.0, 0.0};
+        const Row scaled = {row, vocab, logit_of(key), 1.0 / static_cast<double>(rules.temp), 1.0, 0.0};
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum += scaled.share(l[i]);
     }
@@ -353,13 +383,197 @@ rules_parts_kernel(const float* __restrict__ logits, const float* __restrict__ t
     }
 }
 
-// ---------------------------------------------------------------- second launch
-constexpr int kList = 4096;
+// What the parts say of a row: its largest logit, and the sum of its weights where the row asks for it.
+template <int kBlock>
+struct Whole {
+    static constexpr int kBlockWaves = kBlock / kWave;
+    u64 best[kBlockWaves];
+    double sum[kMaxParts];  // what each part weighs
+
+    __device__ __forceinline__ u64 find_best(const u64* part_best, int parts) {
+        u64 found = 0;
+        for (int q = threadIdx.x; q < parts; q += kBlock) found = part_best[q] > found ? part_best[q] : found;
+#pragma unroll
+        for (int offset = kWave / 2; offset > 0; offset >>= 1) {
+            const u64 other = __shfl_xor(found, offset, kWave);
+            found = other > found ? other : found;
+        }
+        if (threadIdx.x % kWave == 0) best[threadIdx.x / kWave] = found;
+        __syncthreads();
+        for (int w = 0; w < kBlockWaves; ++w) found = best[w] > found ? best[w] : found;
+        return found;
+    }
+    // (in the order of the parts, in every thread)
+    __device__ __forceinline__ double find_total(const Row& row, const u64* part_best, const double* part_sum, int parts) {
+        for (int q = threadIdx.x; q < parts; q += kBlock) {
+            const uint32_t key = static_cast<uint32_t>(part_best[q] >> 32);
+            sum[q] = key > kOrderOfMinusInf ? part_sum[q] * row.share(logit_of(key)) : 0.0;
+        }
+        __syncthreads();
+        double total = 0.0;
+        for (int q = 0; q < parts; ++q) total += sum[q];
+        return total;
+    }
+};
+
+// ---------------------------------------------------------------- rows under top-p or min-p without top-k
+// What weighs less than (1 - p) / vocab of the sum, or less than m, is not kept however the rest is shared out.
+struct Reach {
+    float best;
+    double distance;
+    __device__ __forceinline__ Reach(const Row& row, const Rules& rules, double total) {
+        best = row.best;
+        const double least = rules.p < 1.0 ? fmax((1.0 - rules.p) * total / row.vocab, rules.m) : rules.m;
+        distance = -log(least) * static_cast<double>(rules.temp) * (1.0 + 1e-9) + 1e-30;  // (a little rounded up)
+    }
+    __device__ __forceinline__ bool operator()(float l) const {
+        return l > -INFINITY && (l == best || static_cast<double>(best) - static_cast<double>(l) <= distance);
+    }
+};
+
+// The larger the nearer to the largest.  64 bins to a factor of e; all beyond e^-32 are one, where 8 million tokens together
+// weigh less than the least 1 - p that a float has.
+__device__ __forceinline__ int bin_of(const Row& row, float l) {
+    const double at = l == row.best ? 0.0 : (static_cast<double>(row.best) - static_cast<double>(l)) * row.inv_t * 64.0;
+    return kBins - 1 - (at < kBins - 1 ? static_cast<int>(at) : kBins - 1);
+}
 
 // What a row's numbers are sorted by: the larger logit first, then the lower index.
 __device__ __forceinline__ u64 place_of(float l, int i) { return (static_cast<u64>(~order_of(l)) << 32) | static_cast<uint32_t>(i); }
-__device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
+// Runs f(l, index) over the thread's chunk of a part, if its largest passes.
+template <typename F>
+__device__ __forceinline__ void walk_chunk(const Row& row, const float* chunks, int part, const Reach& reach, F f) {
+    if (!reach(chunks[part * kPartThreads + threadIdx.x])) return;
+    const int first = part * kPart + threadIdx.x * 4;
+    float l[16];
+    const bool lines = (reinterpret_cast<uintptr_t>(row.logits) & 15) == 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int at = first + q * kPartThreads * 4;
+        if (lines && at + 3 < row.vocab) {
+            const float4 v = *reinterpret_cast<const float4*>(row.logits + at);
+            l[q * 4] = v.x;
+            l[q * 4 + 1] = v.y;
+            l[q * 4 + 2] = v.z;
+            l[q * 4 + 3] = v.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) l[q * 4 + e] = at + e < row.vocab ? row.logits[at + e] : -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (reach(l[i])) f(l[i], first + i / 4 * kPartThreads * 4 + i % 4);
+}
+
+// grid: (some workgroups, rows)
+__global__ void __launch_bounds__(kPartThreads)
+rules_tally_kernel(const float* __restrict__ logits, const float* __restrict__ temperature, const int* __restrict__ top_k,
+                   const float* __restrict__ top_p, const float* __restrict__ min_p, PartOf of, int vocab, long ld, int parts, double unit) {
+    __shared__ Whole<kPartThreads> whole;
+    __shared__ u64 s_weight[kBins];
+    const int r = blockIdx.y;
+    const Rules rules(temperature, top_k, top_p, min_p, r, vocab);
+    if (!rules.tallied() || !(rules.p < 1.0)) return;
+    const u64* part_best = of.best + static_cast<size_t>(r) * parts;
+    for (int b = threadIdx.x; b < kBins; b += kPartThreads) s_weight[b] = 0;
+    const uint32_t key = static_cast<uint32_t>(whole.find_best(part_best, parts) >> 32);
+    if (key <= kOrderOfMinusInf) return;
+    const Row row = {logits + static_cast<size_t>(r) * ld, vocab, logit_of(key), 1.0 / static_cast<double>(rules.temp), unit, 0.0};
+    const Reach reach(row, rules, whole.find_total(row, part_best, of.sum + static_cast<size_t>(r) * parts, parts));
+    for (int part = blockIdx.x; part < parts; part += gridDim.x)
+        walk_chunk(row, of.chunk + static_cast<size_t>(r) * parts * kPartThreads, part, reach, [&](float l, int) {
+            const u64 w = row.weight(l);
+            if (w) atomicAdd(&s_weight[bin_of(row, l)], w);
+        });
+    __syncthreads();
+    for (int b = threadIdx.x; b < kBins; b += kPartThreads)
+        if (s_weight[b]) atomicAdd(&of.histogram[static_cast<size_t>(r) * kBins + b], s_weight[b]);
+}
+
+// grid: (some workgroups, rows)
+__global__ void __launch_bounds__(kPartThreads)
+rules_collect_kernel(const float* __restrict__ logits, const float* __restrict__ temperature, const int* __restrict__ top_k,
+                     const float* __restrict__ top_p, const float* __restrict__ min_p, PartOf of, int vocab, long ld, int parts, double unit) {
+    constexpr int kOwn = kBins / kPartThreads, kPartWaves = kPartThreads / kWave;
+    __shared__ Whole<kPartThreads> whole;
+    __shared__ u64 s_sum[kPartWaves];
+    __shared__ int s_bin;
+    __shared__ u64 s_above;
+    const int r = blockIdx.y, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const Rules rules(temperature, top_k, top_p, min_p, r, vocab);
+    if (!rules.tallied()) return;
+    const u64* part_best = of.best + static_cast<size_t>(r) * parts;
+    if (threadIdx.x == 0) {
+        s_bin = -1;
+        s_above = 0;
+    }
+    const uint32_t key = static_cast<uint32_t>(whole.find_best(part_best, parts) >> 32);
+    if (key <= kOrderOfMinusInf) return;
+    const Row row = {logits + static_cast<size_t>(r) * ld, vocab, logit_of(key), 1.0 / static_cast<double>(rules.temp), unit, 0.0};
+    const double total = whole.find_total(row, part_best, of.sum + static_cast<size_t>(r) * parts, parts);
+    const Reach reach(row, rules, total);
+    if (rules.p < 1.0) {
+        // the bin in which p of the weight is reached (without any, the lowest that has weight), and what lies in front of it
+        u64 own[kOwn], mine = 0;
+        const u64* histogram = of.histogram + static_cast<size_t>(r) * kBins;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            own[i] = histogram[kBins - 1 - static_cast<int>(threadIdx.x) * kOwn - i];
+            mine += own[i];
+        }
+        u64 front = wave_running_u64(mine);
+        if (lane == kWave - 1) s_sum[wave] = front;
+        __syncthreads();
+        front -= mine;
+        u64 all = 0;
+        for (int w = 0; w < kPartWaves; ++w) {
+            if (w < wave) front += s_sum[w];
+            all += s_sum[w];
+        }
+        const double limit = fmin(rules.p * total * unit, static_cast<double>(all));
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            // (one bin: what lies in front of it is below the limit, or nothing, and with it the limit is reached)
+            if (own[i] && (front == 0 || static_cast<double>(front) < limit) && static_cast<double>(front + own[i]) >= limit) {
+                s_bin = kBins - 1 - static_cast<int>(threadIdx.x) * kOwn - i;
+                s_above = front;
+            }
+            front += own[i];
+        }
+        __syncthreads();
+    }
+    const int cut_bin = s_bin;  // (-1: all are kept that min-p keeps)
+    if (blockIdx.x == 0 && threadIdx.x == 0) of.head[2 * r + 1] = s_above;
+    u64* list = of.list + static_cast<size_t>(r) * kList;
+    for (int part = blockIdx.x; part < parts; part += gridDim.x) {
+        u64 sum = 0;
+        walk_chunk(row, of.chunk + static_cast<size_t>(r) * parts * kPartThreads, part, reach, [&](float l, int i) {
+            const int bin = bin_of(row, l);
+            if (bin < cut_bin) return;
+            const u64 w = row.weight(l);
+            if (w == 0) return;
+            if (bin > cut_bin) {
+                if (!(rules.m > 0.0 && row.share(l) < rules.m)) sum += w;
+            } else {
+                const u64 at = atomicAdd(&of.head[2 * r], 1ull);
+                if (at < kList) list[at] = place_of(l, i);
+            }
+        });
+        sum = wave_sum_u64(sum);
+        __syncthreads();
+        if (lane == 0) s_sum[wave] = sum;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            sum = 0;
+            for (int w = 0; w < kPartWaves; ++w) sum += s_sum[w];
+            of.kept[static_cast<size_t>(r) * parts + part] = sum;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- last launch
 // list[0 .. n) in ascending order; n up to kList, the list's room up to the next power of two is written.
 __device__ void sort_list(u64* list, int n) {
     int size = 2;
@@ -380,7 +594,7 @@ __device__ void sort_list(u64* list, int n) {
         }
 }
 
-// Running sums in front of list places: thread t has the kList / kThreads places from t * 4 on.
+// Running sums in front of places: thread t has kPlaces of them, from t * kPlaces on.
 constexpr int kPlaces = kList / kThreads;
 __device__ __forceinline__ u64 sums_in_front(const u64 (&own)[kPlaces], u64* s_sum, u64& total) {
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
@@ -399,6 +613,15 @@ __device__ __forceinline__ u64 sums_in_front(const u64 (&own)[kPlaces], u64* s_s
     }
     return front;
 }
+__device__ __forceinline__ u64 block_sum_u64(u64 v, u64* s_sum) {
+    v = wave_sum_u64(v);
+    __syncthreads();
+    if (threadIdx.x % kWave == 0) s_sum[threadIdx.x / kWave] = v;
+    __syncthreads();
+    u64 total = 0;
+    for (int w = 0; w < kWaves; ++w) total += s_sum[w];
+    return total;
+}
 
 // How far down a logit lies, in bins of 1/64 of a power of two: for distances of any scale.
 __device__ __forceinline__ int octave_bin(float distance) {
@@ -407,49 +630,120 @@ __device__ __forceinline__ int octave_bin(float distance) {
 }
 
 struct Shared {
-    Histogram h;
-    u64 list[kList];
-    u64 sum[kWaves], segment[kWaves];
-    int count, kept;
-    int picked;
+    union {
+        Histogram h;
+        int hits[kList];             // chunks that pass
+        u64 weight[kThreads / 4];    // of a short list
+        u64 segment[kMaxParts];      // of the parts
+    };
+    union {
+        u64 list[kList];
+        Whole<kThreads> whole;
+    };
+    u64 sum[kWaves];
+    int count, kept, picked, last;
 };
 
-// The numbers of the row that `passes` takes (it takes all that are larger than one it takes), from the chunks whose largest
-// does; more than kList: as many as there are, and no list.
-template <typename F>
-__device__ int gather_list(const Row& row, const float* chunks, int chunk_count, Shared& s, F passes) {
-    __syncthreads();
-    if (threadIdx.x == 0) s.count = 0;
-    __syncthreads();
-    for (int c = threadIdx.x; c < chunk_count; c += kThreads) {
-        if (!passes(chunks[c])) continue;
-        const int first = c / kPartThreads * kPart + c % kPartThreads * 4;
-        for (int q = 0; q < 4; ++q)
-            for (int e = 0; e < 4; ++e) {
-                const int i = first + q * kPartThreads * 4 + e;
-                if (i >= row.vocab) continue;
-                const float l = row.logits[i];
-                if (!passes(l)) continue;
-                const int at = atomicAdd(&s.count, 1);
-                if (at < kList) s.list[at] = place_of(l, i);
-            }
+// The place whose running sum passes the target, of thread t's kPlaces from t * kPlaces on (`front` in front of them); the last
+// with any weight if none does, -1 without any.
+__device__ __forceinline__ int pick_place(const u64 (&own)[kPlaces], u64 front, double target, Shared& s) {
+    if (threadIdx.x == 0) {
+        s.picked = 0x7fffffff;
+        s.last = -1;
     }
     __syncthreads();
-    return s.count;
+    int mine = -1, last = -1;
+#pragma unroll
+    for (int i = 0; i < kPlaces; ++i) {
+        if (own[i] == 0) continue;
+        last = threadIdx.x * kPlaces + i;
+        front += own[i];
+        if (mine < 0 && static_cast<double>(front) > target) mine = last;
+    }
+    if (mine >= 0) atomicMin(&s.picked, mine);
+    if (last >= 0) atomicMax(&s.last, last);
+    __syncthreads();
+    return s.picked != 0x7fffffff ? s.picked : s.last;
 }
 
-// The draw from a list that holds the first n of the row's order: the first k of them (k = 0: all), then those in front of which
-// less than `limit` lies (or p of what the k weigh, of_list), then min-p.
-__device__ int draw_from_list(const Row& row, Shared& s, int n, int k, bool nucleus, bool of_list, double p_or_limit, double m, double u) {
+// The draw from one part of the row, of what lies up to `cut` in its order; -1 without any weight.
+__device__ int draw_from_part(const Row& row, Shared& s, int part, u64 before, double target, u64 cut) {
+    u64 own[kPlaces], total;
+    const int first = part * kPart + threadIdx.x * kPlaces;
+    static_assert(kPart == kThreads * kPlaces, "a thread has four neighbours of a part");
+#pragma unroll
+    for (int i = 0; i < kPlaces; ++i) {
+        const float l = first + i < row.vocab ? row.logits[first + i] : -INFINITY;
+        own[i] = place_of(l, first + i) <= cut ? row.weight(l) : 0;
+    }
+    const u64 front = before + sums_in_front(own, s.sum, total);
+    const int place = pick_place(own, front, target, s);
+    __syncthreads();
+    return place < 0 ? -1 : part * kPart + place;
+}
+
+// The draw from a list of up to kThreads / 4 numbers that holds the first of the row's order, the first k of them, p, m and u: four
+// threads compare a number with all others, for its rank and what lies in front of it, then for the sum up to its index.
+__device__ int draw_from_few(const Row& row, Shared& s, int n, const Rules& rules, double u) {
+    const int i = threadIdx.x / 4, lane = threadIdx.x % 4;
+    const u64 mine = i < n ? s.list[i] : ~0ull;
+    const float l = logit_of(~static_cast<uint32_t>(mine >> 32));
+    const double share = i < n ? row.share(l) : 0.0;
+    u64 weight = static_cast<u64>(share * row.unit + 0.5);
+    __syncthreads();  // (the histogram and the hits lie where the weights go)
+    if (lane == 0) s.weight[i] = weight;
+    __syncthreads();
+    int rank = 0;
+    u64 front = 0;
+    for (int j = lane; j < n; j += 4)
+        if (s.list[j] < mine) {
+            ++rank;
+            front += s.weight[j];
+        }
+#pragma unroll
+    for (int offset = 1; offset < 4; offset <<= 1) {
+        rank += __shfl_xor(rank, offset, kWave);
+        front += __shfl_xor(front, offset, kWave);
+    }
+    bool kept = i < n && rank < rules.k;
+    if (rules.p < 1.0) {
+        const double limit = rules.p * static_cast<double>(block_sum_u64(kept && lane == 0 ? weight : 0, s.sum));
+        kept = kept && (rank == 0 || static_cast<double>(front) < limit);
+    }
+    kept = kept && (rank == 0 || !(rules.m > 0.0) || share >= rules.m);
+    if (!kept) weight = 0;
+    const double target = u * static_cast<double>(block_sum_u64(lane == 0 ? weight : 0, s.sum));
+    if (lane == 0) s.weight[i] = weight;  // (all have read the old ones: the sum has barriers)
+    if (threadIdx.x == 0) {
+        s.picked = 0x7fffffff;
+        s.last = -1;
+    }
+    __syncthreads();
+    const uint32_t index = static_cast<uint32_t>(mine);
+    u64 running = 0;
+    for (int j = lane; j < n; j += 4)
+        if (static_cast<uint32_t>(s.list[j]) <= index) running += s.weight[j];
+#pragma unroll
+    for (int offset = 1; offset < 4; offset <<= 1) running += __shfl_xor(running, offset, kWave);
+    if (weight) {
+        if (static_cast<double>(running) > target) atomicMin(&s.picked, static_cast<int>(index));
+        atomicMax(&s.last, static_cast<int>(index));
+    }
+    __syncthreads();
+    return s.picked != 0x7fffffff ? s.picked : s.last;
+}
+
+// ... from a longer one.
+__device__ int draw_from_list(const Row& row, Shared& s, int n, const Rules& rules, double u) {
     sort_list(s.list, n);
-    if (k > 0 && k < n) n = k;
+    n = min(n, rules.k);
     u64 own[kPlaces], total;
     const int first = threadIdx.x * kPlaces;
 #pragma unroll
     for (int i = 0; i < kPlaces; ++i)
         own[i] = first + i < n ? row.weight(logit_of(~static_cast<uint32_t>(s.list[first + i] >> 32))) : 0;
     u64 front = sums_in_front(own, s.sum, total);
-    const double limit = of_list ? p_or_limit * static_cast<double>(total) : p_or_limit;
+    const double limit = rules.p * static_cast<double>(total);
     if (threadIdx.x == 0) s.kept = 0;
     __syncthreads();
     int kept = 0;
@@ -457,8 +751,8 @@ __device__ int draw_from_list(const Row& row, Shared& s, int n, int k, bool nucl
     for (int i = 0; i < kPlaces; ++i) {
         if (first + i >= n) break;
         const float l = logit_of(~static_cast<uint32_t>(s.list[first + i] >> 32));
-        if (first + i > 0 && nucleus && !(static_cast<double>(front) < limit)) break;
-        if (first + i > 0 && m > 0.0 && row.share(l) < m) break;
+        if (first + i > 0 && rules.p < 1.0 && !(static_cast<double>(front) < limit)) break;
+        if (first + i > 0 && rules.m > 0.0 && row.share(l) < rules.m) break;
         front += own[i];
         kept = first + i + 1;
     }
@@ -477,108 +771,134 @@ __device__ int draw_from_list(const Row& row, Shared& s, int n, int k, bool nucl
 #pragma unroll
     for (int i = 0; i < kPlaces; ++i) own[i] = first + i < n ? row.weight(logit_of(~static_cast<uint32_t>(s.list[first + i]))) : 0;
     front = sums_in_front(own, s.sum, total);
-    const double target = u * static_cast<double>(total);
-    if (threadIdx.x == 0) s.picked = -1;
-    __syncthreads();
-    // the first place whose running sum passes the target, else the last with any weight
-    int mine = -1, last = -1;
-#pragma unroll
-    for (int i = 0; i < kPlaces; ++i) {
-        if (own[i] == 0) continue;
-        last = first + i;
-        front += own[i];
-        if (mine < 0 && static_cast<double>(front) > target) mine = first + i;
-    }
-    if (mine >= 0) atomicMax(&s.picked, 2 * kList - mine);
-    if (last >= 0) atomicMax(&s.picked, last);
-    __syncthreads();
-    const int place = s.picked >= kList ? 2 * kList - s.picked : s.picked;
+    const int place = pick_place(own, front, u * static_cast<double>(total), s);
     return place < 0 ? -1 : static_cast<int>(s.list[place] >> 32);
 }
 
-// The draw from a share of all weight that is too many tokens for a list: a histogram of the weights over equal bins of
-// (max - l) / T, of which the one that holds the cut goes to the list.  -2: it holds more than the list.
-__device__ int draw_from_row(Row& row, Shared& s, double limit, double m, double u) {
-    constexpr double kBinsOfUnit = 64.0;  // (beyond 32 units, where 2 million tokens weigh less than the least 1 - p, all is one bin)
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const auto bin_of = [&](float l) {
-        const double at = l == row.best ? 0.0 : (static_cast<double>(row.best) - static_cast<double>(l)) * row.inv_t * kBinsOfUnit;
-        return kBins - 1 - (at < kBins - 1 ? static_cast<int>(at) : kBins - 1);
+// The draw under top-k; -2: too many numbers pass the bound.
+__device__ int draw_of_k(const Row& row, Shared& s, const float* chunks, int chunk_count, const Rules& rules, double u) {
+    constexpr int kRound = 16;  // chunks of a thread that are read at once (all of them, up to 262,144 tokens)
+    const auto bin_of = [&](float l) { return kBins - 1 - octave_bin(l == row.best ? 0.f : row.best - l); };
+    const int rounds = (chunk_count + kRound * kThreads - 1) / (kRound * kThreads);
+    float largest[kRound];
+    const auto read = [&](int round) {
+#pragma unroll
+        for (int j = 0; j < kRound; ++j) {
+            const int c = (round * kRound + j) * kThreads + threadIdx.x;
+            largest[j] = c < chunk_count ? chunks[c] : -INFINITY;
+        }
     };
+    read(0);
     for (int b = threadIdx.x; b < kBins; b += kThreads) {
         s.h.weight[b] = 0;
         s.h.count[b] = 0;
     }
+    if (threadIdx.x == 0) s.count = s.kept = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < row.vocab; i += kThreads) {
-        const float l = row.logits[i];
-        const u64 w = row.weight(l);
-        if (w) atomicAdd(&s.h.weight[bin_of(l)], w);
+    for (int round = 0; round < rounds; ++round) {
+        if (round) read(round);
+#pragma unroll
+        for (int j = 0; j < kRound; ++j)
+            if (largest[j] > -INFINITY) atomicAdd(&s.h.count[bin_of(largest[j])], 1);
     }
     __syncthreads();
-    cross(s.h, false, 0, limit);
-    const int cut_bin = s.h.bin;
-    const double above = static_cast<double>(s.h.above_weight);
-    if (threadIdx.x == 0) s.count = 0;
-    if (threadIdx.x < kWaves) s.segment[threadIdx.x] = 0;
+    cross(s.h, true, rules.k, 0.0);  // (fewer chunks than k: the last bin that has any, and then all below it)
+    const int found = s.h.above_count + s.h.count[s.h.bin] >= rules.k ? s.h.bin : -1;
     __syncthreads();
-    const int stretch = ((row.vocab + kWaves - 1) / kWaves + kWave - 1) / kWave * kWave;
-    u64 sum = 0;
-    const int to = min(row.vocab, (wave + 1) * stretch);
-    for (int i = wave * stretch + lane; i < to; i += kWave) {
-        const float l = row.logits[i];
-        const u64 w = row.weight(l);
-        if (w == 0) continue;
-        const int bin = bin_of(l);
-        if (bin > cut_bin) {
-            if (!(m > 0.0 && row.share(l) < m)) sum += w;
-        } else if (bin == cut_bin) {
-            const int at = atomicAdd(&s.count, 1);
-            if (at < kList) s.list[at] = place_of(l, i);
+    const auto passes = [&](float l) { return l > -INFINITY && bin_of(l) >= found; };
+    for (int round = 0; round < rounds; ++round) {
+        if (rounds > 1) read(round);
+#pragma unroll
+        for (int j = 0; j < kRound; ++j)
+            if (passes(largest[j])) {
+                const int at = atomicAdd(&s.kept, 1);
+                if (at < kList) s.hits[at] = (round * kRound + j) * kThreads + threadIdx.x;
+            }
+    }
+    __syncthreads();
+    const int hits = s.kept;
+    if (hits > kList) return -2;  // (each has a number that passes)
+    const bool lines = (reinterpret_cast<uintptr_t>(row.logits) & 15) == 0;
+    for (int item = threadIdx.x; item < hits * 4; item += kThreads) {
+        const int c = s.hits[item / 4], first = c / kPartThreads * kPart + c % kPartThreads * 4 + item % 4 * kPartThreads * 4;
+        float l[4];
+        if (lines && first + 3 < row.vocab) {
+            const float4 v = *reinterpret_cast<const float4*>(row.logits + first);
+            l[0] = v.x;
+            l[1] = v.y;
+            l[2] = v.z;
+            l[3] = v.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) l[e] = first + e < row.vocab ? row.logits[first + e] : -INFINITY;
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (passes(l[e])) {
+                const int at = atomicAdd(&s.count, 1);
+                if (at < kList) s.list[at] = place_of(l[e], first + e);
+            }
     }
-    sum = wave_sum_u64(sum);
-    if (lane == 0) s.segment[wave] = sum;
     __syncthreads();
     const int n = s.count;
     if (n > kList) return -2;
-    sort_list(s.list, n);
-    u64 own[kPlaces], total;
-    const int first = threadIdx.x * kPlaces;
-#pragma unroll
-    for (int i = 0; i < kPlaces; ++i)
-        own[i] = first + i < n ? row.weight(logit_of(~static_cast<uint32_t>(s.list[first + i] >> 32))) : 0;
-    u64 front = sums_in_front(own, s.sum, total);
-    if (threadIdx.x == 0) s.kept = 0;
-    __syncthreads();
-    row.least = m;
-#pragma unroll
-    for (int i = 0; i < kPlaces; ++i) {
-        if (first + i >= n || !(first + i == 0 && above == 0.0) && !(above + static_cast<double>(front) < limit)) break;
-        front += own[i];
-        atomicMax(&s.kept, first + i + 1);
-        const u64 w = row.weight(logit_of(~static_cast<uint32_t>(s.list[first + i] >> 32)));
-        if (w) atomicAdd(&s.segment[static_cast<uint32_t>(s.list[first + i]) / stretch], w);
-    }
-    __syncthreads();
-    // (nothing of the bin is kept only if rounding says so: then the cut lies in front of it)
-    const u64 last = s.kept > 0 ? s.list[s.kept - 1] : n > 0 ? s.list[0] - 1 : 0;
+    return n <= kThreads / 4 ? draw_from_few(row, s, n, rules, u) : draw_from_list(row, s, n, rules, u);
+}
+
+// The part in which the running sum of s.segment passes u times the whole, and its draw.
+__device__ int draw_from_segments(const Row& row, Shared& s, int parts, double u, u64 cut) {
+    // (every thread goes through them: a wave would have to tell the others what it found)
     u64 all = 0;
-    for (int w = 0; w < kWaves; ++w) all += s.segment[w];
+    for (int q = 0; q < parts; ++q) all += s.segment[q];
     const double target = u * static_cast<double>(all);
     int owner = 0;
     u64 running = 0, before = 0;
-    for (int w = 0; w < kWaves; ++w) {
-        if (s.segment[w] == 0) continue;
-        owner = w;
+    for (int q = 0; q < parts; ++q) {
+        if (s.segment[q] == 0) continue;
+        owner = q;
         before = running;
-        running += s.segment[w];
+        running += s.segment[q];
         if (static_cast<double>(running) > target) break;
     }
-    return seek(owner * stretch, min(row.vocab, (owner + 1) * stretch), before, target, false, s.sum, [&](int i) -> u64 {
-        const float l = row.logits[i];
-        return place_of(l, i) <= last ? row.weight(l) : 0;
-    });
+    return draw_from_part(row, s, owner, before, target, cut);
+}
+
+// The draw of a row that was tallied; -2: the cut's bin holds more than its list.
+__device__ int draw_of_tally(Row& row, Shared& s, const PartOf& of, int r, int parts, const Rules& rules, double total, double u) {
+    const u64 listed = of.head[2 * r], above = of.head[2 * r + 1];
+    if (rules.p < 1.0 && listed > kList) return -2;
+    const int n = rules.p < 1.0 ? static_cast<int>(listed) : 0;
+    const double limit = rules.p * total * row.unit;
+    for (int q = threadIdx.x; q < parts; q += kThreads) s.segment[q] = of.kept[static_cast<size_t>(r) * parts + q];
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) s.list[i] = of.list[static_cast<size_t>(r) * kList + i];
+    u64 cut = ~0ull;  // the last kept place
+    if (rules.p < 1.0) {
+        sort_list(s.list, n);
+        u64 own[kPlaces], weight;
+        const int first = threadIdx.x * kPlaces;
+#pragma unroll
+        for (int i = 0; i < kPlaces; ++i)
+            own[i] = first + i < n ? row.weight(logit_of(~static_cast<uint32_t>(s.list[first + i] >> 32))) : 0;
+        u64 front = above + sums_in_front(own, s.sum, weight);
+        if (threadIdx.x == 0) s.kept = 0;
+        __syncthreads();
+        row.least = rules.m;
+#pragma unroll
+        for (int i = 0; i < kPlaces; ++i) {
+            if (first + i >= n || !(front == 0 || static_cast<double>(front) < limit)) break;
+            front += own[i];
+            atomicMax(&s.kept, first + i + 1);
+            const u64 w = row.weight(logit_of(~static_cast<uint32_t>(s.list[first + i] >> 32)));
+            if (w) atomicAdd(&s.segment[static_cast<uint32_t>(s.list[first + i]) / kPart], w);
+        }
+        __syncthreads();
+        // (nothing of the bin is kept only if rounding says so: the cut then lies right in front of it)
+        cut = s.kept > 0 ? s.list[s.kept - 1] : n > 0 ? s.list[0] - 1 : ~0ull;
+        __syncthreads();
+    }
+    row.least = rules.m;
+    return draw_from_segments(row, s, parts, u, cut);
 }
 
 __global__ void __launch_bounds__(kThreads)
@@ -586,106 +906,61 @@ rules_draw_kernel(const float* __restrict__ logits, const float* __restrict__ te
                   const int* __restrict__ top_k, const float* __restrict__ top_p, const float* __restrict__ min_p, PartOf of,
                   int* __restrict__ out, int vocab, long ld, int parts, double unit) {
     __shared__ Shared s;
-    const int r = blockIdx.x, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int r = blockIdx.x;
     const u64* part_best = of.best + static_cast<size_t>(r) * parts;
-    const double* part_sum = of.sum + static_cast<size_t>(r) * parts;
-    const float* chunks = of.chunk + static_cast<size_t>(r) * parts * kPartThreads;
-
-    // the largest logit and its first index
-    u64 best = 0;
-    for (int p = threadIdx.x; p < parts; p += kThreads) best = part_best[p] > best ? part_best[p] : best;
-#pragma unroll
-    for (int offset = kWave / 2; offset > 0; offset >>= 1) {
-        const u64 other = __shfl_xor(best, offset, kWave);
-        best = other > best ? other : best;
-    }
-    if (lane == 0) s.sum[wave] = best;
-    __syncthreads();
-    for (int w = 0; w < kWaves; ++w) best = s.sum[w] > best ? s.sum[w] : best;
-    __syncthreads();
+    const Rules rules(temperature, top_k, top_p, min_p, r, vocab);
+    const u64 best = s.whole.find_best(part_best, parts);
     const uint32_t best_key = static_cast<uint32_t>(best >> 32);
     const int best_idx = best_key > kOrderOfMinusInf ? 0x7fffffff - static_cast<int>(best & 0xffffffffu) : 0;
-    const float temp = temperature[r];
-    if (!(temp > 0.f) || best_key <= kOrderOfMinusInf) {
+    if (!rules.draws() || best_key <= kOrderOfMinusInf) {
         if (threadIdx.x == 0) out[r] = best_idx;
         return;
     }
-    Row row = {logits + static_cast<size_t>(r) * ld, vocab, logit_of(best_key), 1.0 / static_cast<double>(temp), unit, 0.0};
-    const int k = top_k && top_k[r] > 0 && top_k[r] < vocab ? top_k[r] : 0;
-    const double p = top_p && top_p[r] < 1.f ? (top_p[r] > 0.f ? static_cast<double>(top_p[r]) : 0.0) : 1.0;  // (NaN: off)
-    const double m = min_p && min_p[r] > 0.f ? (min_p[r] < 1.f ? static_cast<double>(min_p[r]) : 1.0) : 0.0;  // (the largest stays)
+    Row row = {logits + static_cast<size_t>(r) * ld, vocab, logit_of(best_key), 1.0 / static_cast<double>(rules.temp), unit, 0.0};
     const double u = static_cast<double>(uniform[r]);
-    const int chunk_count = parts * kPartThreads;
-
+    __syncthreads();
     int picked = -2;
-    if (k > 0) {
-        for (int b = threadIdx.x; b < kBins; b += kThreads) {
-            s.h.weight[b] = 0;
-            s.h.count[b] = 0;
-        }
-        __syncthreads();
-        const auto bin_of = [&](float l) { return kBins - 1 - octave_bin(l == row.best ? 0.f : row.best - l); };
-        for (int c = threadIdx.x; c < chunk_count; c += kThreads)
-            if (chunks[c] > -INFINITY) atomicAdd(&s.h.count[bin_of(chunks[c])], 1);
-        __syncthreads();
-        cross(s.h, true, k, 0.0);  // (fewer chunks than k: the last bin that has any, and then all below it)
-        const int found = s.h.bin;
-        const bool enough = s.h.above_count + s.h.count[found] >= k;
-        const int n = gather_list(row, chunks, chunk_count, s, [&](float l) { return l > -INFINITY && (!enough || bin_of(l) >= found); });
-        if (n <= kList) picked = draw_from_list(row, s, n, k, p < 1.0, true, p, m, u);
+    if (rules.k > 0) {
+        picked = draw_of_k(row, s, of.chunk + static_cast<size_t>(r) * parts * kPartThreads, parts * kPartThreads, rules, u);
     } else {
-        double total = 0.0, owner_before = 0.0;
-        int owner = 0;
-        double* const part = reinterpret_cast<double*>(s.list);  // what each part weighs
-        for (int q = threadIdx.x; q < parts; q += kThreads) {
-            const uint32_t key = static_cast<uint32_t>(part_best[q] >> 32);
-            part[q] = key > kOrderOfMinusInf ? part_sum[q] * row.share(logit_of(key)) : 0.0;
-        }
-        __syncthreads();
-        for (int q = 0; q < parts; ++q) total += part[q];  // (in order, in every thread)
-        // what weighs less than this is not kept, however it is shared out; as a distance from the largest, a little rounded up
-        const double least = p < 1.0 ? fmax((1.0 - p) * total / vocab, m) : m;
-        if (least > 0.0) {
-            const double reach = -log(least) * static_cast<double>(temp) * (1.0 + 1e-9) + 1e-30;
-            const auto passes = [&](float l) {
-                return l > -INFINITY && (l == row.best || static_cast<double>(row.best) - static_cast<double>(l) <= reach);
-            };
-            const int n = gather_list(row, chunks, chunk_count, s, passes);
-            if (n <= kList)
-                picked = draw_from_list(row, s, n, 0, p < 1.0, false, p * total * unit, m, u);
-            else if (p < 1.0)
-                picked = draw_from_row(row, s, p * total * unit, m, u);
-            else {
-                row.least = m;
-                picked = seek(0, vocab, 0, u, true, s.sum, [&](int i) -> u64 { return row.weight(row.logits[i]); });
-            }
+        const double total = s.whole.find_total(row, part_best, of.sum + static_cast<size_t>(r) * parts, parts);
+        if (rules.tallied()) {
+            __syncthreads();
+            picked = draw_of_tally(row, s, of, r, parts, rules, total, u);
         } else {
             const double target = u * total;
-            double running = 0.0;
+            int owner = 0;
+            double running = 0.0, before = 0.0;
             for (int q = 0; q < parts; ++q) {
-                if (part[q] * unit < 0.5) continue;
+                const double mine = s.whole.sum[q];
+                if (mine * unit < 0.5) continue;
                 owner = q;
-                owner_before = running;
-                running += part[q];
+                before = running;
+                running += mine;
                 if (running > target) break;
             }
             // (a part whose numbers each round to no weight has nothing to draw: the next one then)
             picked = -1;
             for (int q = owner; q < parts && picked < 0; ++q)
-                picked = seek(q * kPart, min(vocab, (q + 1) * kPart), 0, q == owner ? (target - owner_before) * unit : -1.0, false, s.sum,
-                              [&](int i) -> u64 { return row.weight(row.logits[i]); });
+                picked = draw_from_part(row, s, q, 0, q == owner ? (target - before) * unit : -1.0, ~0ull);
         }
     }
-    if (picked == -2) picked = draw_by_bits(row, s.h, s.sum, k, p, m, u);
+    if (picked == -2) {
+        __syncthreads();
+        row.least = 0.0;
+        picked = draw_by_bits(row, s.h, s.sum, rules.k, rules.p, rules.m, u);
+    }
     if (threadIdx.x == 0) out[r] = picked < 0 ? best_idx : picked;
 }
 
 }  // namespace
 
-// top_k, top_p and min_p may each be null: that rule is off in every row.  work: rows * ceil(vocab / 4096) * 1040 bytes, aligned to 8.
+// top_k, top_p and min_p may each be null: that rule is off in every row.  work, aligned to 8 bytes: rows * ceil(vocab / 4096) * 1,048
+// bytes, and rows * 49,168 behind them where top_p or min_p is given.  spread: the workgroups that share a row under these.
 CIE_API int cie_sample_rules(void* stream, const float* logits, const float* temperature, const float* uniform, const int* top_k,
-                             const float* top_p, const float* min_p, int* out, void* work, int rows, int vocab, long ld) {
-    if (rows < 0 || vocab <= 0 || ld < vocab || rows > 65535 || vocab > kList * kPart || !logits || !temperature || !uniform || !out || !work)
+                             const float* top_p, const float* min_p, int* out, void* work, int rows, int vocab, long ld, int spread) {
+    if (rows < 0 || vocab <= 0 || ld < vocab || rows > 65535 || vocab > kMaxParts * kPart || spread < 1 || !logits || !temperature ||
+        !uniform || !out || !work)
         return CIE_BAD_ARGUMENT;
     if (rows == 0) return CIE_OK;
     int bits = 0;
@@ -696,10 +971,23 @@ CIE_API int cie_sample_rules(void* stream, const float* logits, const float* tem
     PartOf of;
     of.best = static_cast<u64*>(work);
     of.sum = reinterpret_cast<double*>(of.best + all);
-    of.chunk = reinterpret_cast<float*>(of.sum + all);
+    of.kept = reinterpret_cast<u64*>(of.sum + all);
+    of.chunk = reinterpret_cast<float*>(of.kept + all);
+    of.histogram = reinterpret_cast<u64*>(of.chunk + all * kPartThreads);
+    of.list = of.histogram + static_cast<size_t>(rows) * kBins;
+    of.head = of.list + static_cast<size_t>(rows) * kList;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    rules_parts_kernel<<<dim3(parts, rows), kPartThreads, 0, s>>>(logits, temperature, top_k, of, vocab, ld);
+    rules_parts_kernel<<<dim3(parts, rows), kPartThreads, 0, s>>>(logits, temperature, top_k, top_p, min_p, of, vocab, ld);
     if (cie_after_launch() != CIE_OK) return CIE_LAUNCH_FAILED;
+    if (top_p || min_p) {
+        const dim3 grid(spread < parts ? spread : parts, rows);
+        if (top_p) {
+            rules_tally_kernel<<<grid, kPartThreads, 0, s>>>(logits, temperature, top_k, top_p, min_p, of, vocab, ld, parts, unit);
+            if (cie_after_launch() != CIE_OK) return CIE_LAUNCH_FAILED;
+        }
+        rules_collect_kernel<<<grid, kPartThreads, 0, s>>>(logits, temperature, top_k, top_p, min_p, of, vocab, ld, parts, unit);
+        if (cie_after_launch() != CIE_OK) return CIE_LAUNCH_FAILED;
+    }
     rules_draw_kernel<<<rows, kThreads, 0, s>>>(logits, temperature, uniform, top_k, top_p, min_p, of, out, vocab, ld, parts, unit);
     return cie_after_launch();
 }

@@ -1504,8 +1504,10 @@ def _per_row(name: str, t: torch.Tensor, dtype: torch.dtype, rows: int) -> None:
         raise ValueError(f"{name} must be [{rows}], is {list(t.shape)}")
 
 
-MAX_RULE_ROWS, MAX_RULE_VOCAB = 65535, 1 << 24
-RULES_PART = 4096  # logits of a part of the first launch, whose results take 130 words of 8 bytes
+MAX_RULE_ROWS, MAX_RULE_VOCAB = 65535, 1 << 23
+# The workspace of a draw under rules, in words of 8 bytes: for each part of so many logits, and for a row's histogram and list
+RULES_PART, RULES_PART_WORDS, RULES_ROW_WORDS = 4096, 131, 2048 + 4096 + 2
+RULES_SPREAD = 2048  # workgroups of a launch in which rows without top-p and min-p have nothing to do
 
 
 def _sample_rules(logits, temperature, uniform, out, top_k, top_p, min_p) -> torch.Tensor:
@@ -1525,10 +1527,13 @@ def _sample_rules(logits, temperature, uniform, out, top_k, top_p, min_p) -> tor
     _on_current_gpu(logits, temperature, uniform, top_k, top_p, min_p, out)
     if rows == 0:
         return out
-    work = torch.empty(rows * -(-vocab // RULES_PART) * 130, dtype=torch.int64, device=logits.device)
+    words = RULES_PART_WORDS * -(-vocab // RULES_PART)
+    if top_p is not None or min_p is not None:
+        words += RULES_ROW_WORDS
+    work = torch.empty(rows * words, dtype=torch.int64, device=logits.device)
     _run("cie_sample_rules", load_library().cie_sample_rules(
         _stream(), _ptr(logits), _ptr(temperature), _ptr(uniform), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(out), _ptr(work),
-        _i(rows), _i(vocab), _i(_ld(logits))))
+        _i(rows), _i(vocab), _i(_ld(logits)), _i(max(1, RULES_SPREAD // rows))))
     return out
 
 
