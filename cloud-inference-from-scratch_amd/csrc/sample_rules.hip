@@ -65,20 +65,45 @@ struct Row {
     }
 };
 
-__device__ __forceinline__ u64 wave_sum_u64(u64 v) {
+// 64-bit sums over a wave without a round trip through LDS a step (a dozen of them were most of what a row's last launch took).
+__device__ __forceinline__ u64 joined(uint32_t lo, uint32_t hi) { return static_cast<u64>(hi) << 32 | lo; }
+template <int kControl, int kRows>
+__device__ __forceinline__ u64 moved(u64 v) {  // (0 where a lane has no source, or lies in a row of 16 that is left out)
+    const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v & 0xffffffffu), kControl, kRows, 0xf, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), kControl, kRows, 0xf, false);
+    return joined(static_cast<uint32_t>(lo), static_cast<uint32_t>(hi));
+}
+// The sum of the lanes up to each one: 1, 2, 4 and 8 lanes on within rows of 16, then a row's last lane to the next row, and the
+// second row's to the upper half.
+__device__ __forceinline__ u64 wave_running_u64(u64 v) {
+    v += moved<0x111, 0xf>(v);
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);
+    return v + moved<0x143, 0xc>(v);
+}
+__device__ __forceinline__ u64 last_lane(u64 v) {
+    return joined(__builtin_amdgcn_readlane(static_cast<int>(v & 0xffffffffu), kWave - 1),
+                  __builtin_amdgcn_readlane(static_cast<int>(v >> 32), kWave - 1));
+}
+__device__ __forceinline__ u64 wave_sum_u64(u64 v) { return last_lane(wave_running_u64(v)); }
+__device__ __forceinline__ u64 wave_most_u64(u64 v) {
 #pragma unroll
-    for (int offset = kWave / 2; offset > 0; offset >>= 1) v += __shfl_xor(v, offset, kWave);
+    for (int offset = kWave / 2; offset > 0; offset >>= 1) {
+        const u64 other = __shfl_xor(v, offset, kWave);
+        v = other > v ? other : v;
+    }
     return v;
 }
 
-__device__ __forceinline__ u64 wave_running_u64(u64 v) {
-    const int lane = threadIdx.x % kWave;
-#pragma unroll
-    for (int offset = 1; offset < kWave; offset <<= 1) {
-        const u64 below = __shfl_up(v, offset, kWave);
-        if (lane >= offset) v += below;
-    }
-    return v;
+// What the waves of a workgroup left in `s` (kCount of them): the sum of those in front of this one, and of all.
+template <int kCount>
+__device__ __forceinline__ void across_waves(const u64* s, u64& front, u64& total) {
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const u64 own = lane < kCount ? s[lane] : 0;
+    front = wave_sum_u64(lane < wave ? own : 0);
+    total = wave_sum_u64(own);
 }
 
 // The first index of [begin, end) whose running sum of f(i), with `before` in front of it, passes the target (u times the whole
@@ -125,62 +150,35 @@ __device__ int seek(int begin, int end, u64 before, double target, bool of_whole
 struct Histogram {
     u64 weight[kBins];
     int count[kBins];
-    u64 wave_weight[kWaves];
-    int wave_count[kWaves];
+    u64 wave[kWaves];
     int bin;
-    u64 above_weight;
-    int above_count;
+    u64 above;
 };
 
 // The bin, from the largest digit down, in which the running count reaches `need` (by_count), or the running weight `limit`;
-// the last bin that counts (weighs) anything if none does.  The sums of the bins in front of it are left in `h`.
-__device__ void cross(Histogram& h, bool by_count, int need, double limit) {
+// the last bin that counts (weighs) anything if none does, -1 if all are empty.  The sum of the bins in front of it is left in
+// h.above, the bin in h.bin.
+template <bool kByCount>
+__device__ void cross(Histogram& h, int need, double limit) {
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     // thread t has bins kBins - 1 - 2 t and the next lower one
     const int hi = kBins - 1 - 2 * threadIdx.x, lo = hi - 1;
-    const u64 own_w = h.weight[hi] + h.weight[lo];
-    const int own_c = h.count[hi] + h.count[lo];
-    u64 run_w = wave_running_u64(own_w);
-    int run_c = own_c;
-#pragma unroll
-    for (int offset = 1; offset < kWave; offset <<= 1) {
-        const int below = __shfl_up(run_c, offset, kWave);
-        if (lane >= offset) run_c += below;
-    }
-    if (lane == kWave - 1) {
-        h.wave_weight[wave] = run_w;
-        h.wave_count[wave] = run_c;
-    }
+    const u64 in_hi = kByCount ? static_cast<u64>(h.count[hi]) : h.weight[hi], in_lo = kByCount ? static_cast<u64>(h.count[lo]) : h.weight[lo];
+    const u64 running = wave_running_u64(in_hi + in_lo);
+    if (lane == kWave - 1) h.wave[wave] = running;
     if (threadIdx.x == 0) h.bin = -1;
     __syncthreads();
-    for (int w = 0; w < wave; ++w) {
-        run_w += h.wave_weight[w];
-        run_c += h.wave_count[w];
-    }
-    u64 before_w = run_w - own_w;
-    int before_c = run_c - own_c;
-    for (int i = 0; i < 2; ++i) {
-        const int bin = i == 0 ? hi : lo;
-        const u64 after_w = before_w + h.weight[bin];
-        const int after_c = before_c + h.count[bin];
-        const bool reached = by_count ? after_c >= need : static_cast<double>(after_w) >= limit;
-        if (reached && (by_count ? h.count[bin] > 0 : h.weight[bin] > 0)) atomicMax(&h.bin, bin);
-        before_w = after_w;
-        before_c = after_c;
-    }
-    __syncthreads();
-    int found = h.bin;
-    __syncthreads();
-    if (found < 0) {  // (a limit that rounding left out of reach)
-        const bool low = by_count ? h.count[lo] > 0 : h.weight[lo] > 0, high = by_count ? h.count[hi] > 0 : h.weight[hi] > 0;
-        if (low || high) atomicMax(&h.bin, kBins - (low ? lo : hi));
-        __syncthreads();
-        found = kBins - h.bin;
-    }
-    if (found == hi || found == lo) {
-        h.bin = found;
-        h.above_weight = run_w - own_w + (found == lo ? h.weight[hi] : 0);
-        h.above_count = run_c - own_c + (found == lo ? h.count[hi] : 0);
+    u64 front, total;
+    across_waves<kWaves>(h.wave, front, total);
+    front += running - in_hi - in_lo;
+    // (one bin: what lies in front of it does not reach, or is nothing, and with it the sum does)
+    const double wanted = fmin(kByCount ? static_cast<double>(need) : limit, static_cast<double>(total));
+    const bool in_first = in_hi && (front == 0 || static_cast<double>(front) < wanted) && static_cast<double>(front + in_hi) >= wanted;
+    const bool in_second = in_lo && (front + in_hi == 0 || static_cast<double>(front + in_hi) < wanted) &&
+                           static_cast<double>(front + in_hi + in_lo) >= wanted;
+    if (in_first || in_second) {
+        h.bin = in_first ? hi : lo;
+        h.above = front + (in_first ? 0 : in_hi);
     }
     __syncthreads();
 }
@@ -216,10 +214,24 @@ __device__ Cut find_cut(const Row& row, Histogram& h, bool by_count, int need, d
             if (w) atomicAdd(&h.weight[bin], w);
         }
         __syncthreads();
-        cross(h, by_count, cut.ties, limit - static_cast<double>(cut.above));
+        if (by_count)
+            cross<true>(h, cut.ties, 0.0);
+        else
+            cross<false>(h, 0, limit - static_cast<double>(cut.above));
         cut.key |= static_cast<uint32_t>(h.bin) << shift;
-        cut.above += h.above_weight;
-        if (by_count) cut.ties -= h.above_count;
+        if (by_count) {  // (what the larger bins weigh: the sum that decided is their count)
+            u64 above = 0;
+            for (int b = threadIdx.x; b < kBins; b += kThreads) above += b > h.bin ? h.weight[b] : 0;
+            above = wave_sum_u64(above);
+            if (threadIdx.x % kWave == 0) h.wave[threadIdx.x / kWave] = above;
+            __syncthreads();
+            u64 front;
+            across_waves<kWaves>(h.wave, front, above);
+            cut.above += above;
+            cut.ties -= static_cast<int>(h.above);
+        } else {
+            cut.above += h.above;
+        }
         cut.equal = h.count[h.bin];
         cut.each = h.weight[h.bin];
     }
@@ -393,17 +405,12 @@ struct Whole {
     __device__ __forceinline__ u64 find_best(const u64* part_best, int parts) {
         u64 found = 0;
         for (int q = threadIdx.x; q < parts; q += kBlock) found = part_best[q] > found ? part_best[q] : found;
-#pragma unroll
-        for (int offset = kWave / 2; offset > 0; offset >>= 1) {
-            const u64 other = __shfl_xor(found, offset, kWave);
-            found = other > found ? other : found;
-        }
+        found = wave_most_u64(found);
         if (threadIdx.x % kWave == 0) best[threadIdx.x / kWave] = found;
         __syncthreads();
-        for (int w = 0; w < kBlockWaves; ++w) found = best[w] > found ? best[w] : found;
-        return found;
+        return wave_most_u64(best[threadIdx.x % kBlockWaves]);
     }
-    // (in the order of the parts, in every thread)
+    // (every wave the same: lanes take the parts in turn, and are added in one order)
     __device__ __forceinline__ double find_total(const Row& row, const u64* part_best, const double* part_sum, int parts) {
         for (int q = threadIdx.x; q < parts; q += kBlock) {
             const uint32_t key = static_cast<uint32_t>(part_best[q] >> 32);
@@ -411,7 +418,9 @@ struct Whole {
         }
         __syncthreads();
         double total = 0.0;
-        for (int q = 0; q < parts; ++q) total += sum[q];
+        for (int q = threadIdx.x % kWave; q < parts; q += kWave) total += sum[q];
+#pragma unroll
+        for (int offset = kWave / 2; offset > 0; offset >>= 1) total += __shfl_xor(total, offset, kWave);
         return total;
     }
 };
@@ -499,8 +508,8 @@ rules_collect_kernel(const float* __restrict__ logits, const float* __restrict__
     constexpr int kOwn = kBins / kPartThreads, kPartWaves = kPartThreads / kWave;
     __shared__ Whole<kPartThreads> whole;
     __shared__ u64 s_sum[kPartWaves];
-    __shared__ int s_bin;
-    __shared__ u64 s_above;
+    __shared__ int s_bin, s_count;
+    __shared__ u64 s_above, s_at, s_list[kPart];
     const int r = blockIdx.y, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const Rules rules(temperature, top_k, top_p, min_p, r, vocab);
     if (!rules.tallied()) return;
@@ -523,15 +532,12 @@ rules_collect_kernel(const float* __restrict__ logits, const float* __restrict__
             own[i] = histogram[kBins - 1 - static_cast<int>(threadIdx.x) * kOwn - i];
             mine += own[i];
         }
-        u64 front = wave_running_u64(mine);
-        if (lane == kWave - 1) s_sum[wave] = front;
+        const u64 running = wave_running_u64(mine);
+        if (lane == kWave - 1) s_sum[wave] = running;
         __syncthreads();
-        front -= mine;
-        u64 all = 0;
-        for (int w = 0; w < kPartWaves; ++w) {
-            if (w < wave) front += s_sum[w];
-            all += s_sum[w];
-        }
+        u64 front, all;
+        across_waves<kPartWaves>(s_sum, front, all);
+        front += running - mine;
         const double limit = fmin(rules.p * total * unit, static_cast<double>(all));
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) {
@@ -548,6 +554,8 @@ rules_collect_kernel(const float* __restrict__ logits, const float* __restrict__
     if (blockIdx.x == 0 && threadIdx.x == 0) of.head[2 * r + 1] = s_above;
     u64* list = of.list + static_cast<size_t>(r) * kList;
     for (int part = blockIdx.x; part < parts; part += gridDim.x) {
+        if (threadIdx.x == 0) s_count = 0;
+        __syncthreads();
         u64 sum = 0;
         walk_chunk(row, of.chunk + static_cast<size_t>(r) * parts * kPartThreads, part, reach, [&](float l, int i) {
             const int bin = bin_of(row, l);
@@ -557,41 +565,76 @@ rules_collect_kernel(const float* __restrict__ logits, const float* __restrict__
             if (bin > cut_bin) {
                 if (!(rules.m > 0.0 && row.share(l) < rules.m)) sum += w;
             } else {
-                const u64 at = atomicAdd(&of.head[2 * r], 1ull);
-                if (at < kList) list[at] = place_of(l, i);
+                s_list[atomicAdd(&s_count, 1)] = place_of(l, i);
             }
         });
         sum = wave_sum_u64(sum);
-        __syncthreads();
         if (lane == 0) s_sum[wave] = sum;
         __syncthreads();
+        u64 front;
+        across_waves<kPartWaves>(s_sum, front, sum);
+        const int count = s_count;
         if (threadIdx.x == 0) {
-            sum = 0;
-            for (int w = 0; w < kPartWaves; ++w) sum += s_sum[w];
             of.kept[static_cast<size_t>(r) * parts + part] = sum;
+            if (count) s_at = atomicAdd(&of.head[2 * r], static_cast<u64>(count));  // (the order in the list changes nothing)
         }
+        __syncthreads();
+        for (int i = threadIdx.x; i < count; i += kPartThreads)
+            if (s_at + i < kList) list[s_at + i] = s_list[i];
     }
 }
 
 // ---------------------------------------------------------------- last launch
-// list[0 .. n) in ascending order; n up to kList, the list's room up to the next power of two is written.
+// list[0 .. n) in ascending order; n up to kList, the list's room up to the next power of two is written.  A thread holds kOwn
+// neighbours: numbers that are compared lie in one thread, in one wave, or pass through LDS.
+template <int kOwn>
+__device__ void sort_held(u64* list, int n, int size) {
+    u64 own[kOwn];
+    const int first = threadIdx.x * kOwn;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) own[i] = first + i < n ? list[first + i] : ~0ull;
+    for (int run = 2; run <= size; run <<= 1) {
+        for (int apart = run >> 1; apart > 0; apart >>= 1) {
+            u64 other[kOwn];
+            if (apart >= kOwn * kWave) {
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i)
+                    if (first + i < size) list[first + i] = own[i];
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i) other[i] = first + i < size ? list[(first + i) ^ apart] : ~0ull;
+            } else if (apart >= kOwn) {
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i) other[i] = __shfl_xor(own[i], apart / kOwn, kWave);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i) other[i] = apart == 1 ? own[i ^ 1] : own[(i ^ 2) % kOwn];
+            }
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i) {
+                const int at = first + i;
+                const bool low = (at & apart) == 0, up = (at & run) == 0;
+                if ((own[i] > other[i]) == (low == up)) own[i] = other[i];
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i)
+        if (first + i < size) list[first + i] = own[i];
+    __syncthreads();
+}
 __device__ void sort_list(u64* list, int n) {
     int size = 2;
     while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += kThreads) list[i] = ~0ull;
     __syncthreads();
-    for (int run = 2; run <= size; run <<= 1)
-        for (int apart = run >> 1; apart > 0; apart >>= 1) {
-            for (int t = threadIdx.x; t < size / 2; t += kThreads) {
-                const int i = 2 * t - (t & (apart - 1)), j = i + apart;
-                const u64 a = list[i], b = list[j];
-                if ((a > b) == ((i & run) == 0)) {
-                    list[i] = b;
-                    list[j] = a;
-                }
-            }
-            __syncthreads();
-        }
+    if (size <= kThreads)
+        sort_held<1>(list, n, size);
+    else if (size <= 2 * kThreads)
+        sort_held<2>(list, n, size);
+    else
+        sort_held<4>(list, n, size);
 }
 
 // Running sums in front of places: thread t has kPlaces of them, from t * kPlaces on.
@@ -605,21 +648,17 @@ __device__ __forceinline__ u64 sums_in_front(const u64 (&own)[kPlaces], u64* s_s
     __syncthreads();
     if (lane == kWave - 1) s_sum[wave] = running;
     __syncthreads();
-    u64 front = running - mine;
-    total = 0;
-    for (int w = 0; w < kWaves; ++w) {
-        if (w < wave) front += s_sum[w];
-        total += s_sum[w];
-    }
-    return front;
+    u64 front;
+    across_waves<kWaves>(s_sum, front, total);
+    return front + running - mine;
 }
 __device__ __forceinline__ u64 block_sum_u64(u64 v, u64* s_sum) {
     v = wave_sum_u64(v);
     __syncthreads();
     if (threadIdx.x % kWave == 0) s_sum[threadIdx.x / kWave] = v;
     __syncthreads();
-    u64 total = 0;
-    for (int w = 0; w < kWaves; ++w) total += s_sum[w];
+    u64 front, total;
+    across_waves<kWaves>(s_sum, front, total);
     return total;
 }
 
@@ -641,29 +680,42 @@ struct Shared {
         Whole<kThreads> whole;
     };
     u64 sum[kWaves];
-    int count, kept, picked, last;
+    int count, hit_count, picked[kWaves], last[kWaves];
 };
+
+// The smallest of the threads' first choices (0x7fffffff: none), the largest of their second ones (-1) if there is none.
+__device__ __forceinline__ int choose(int first, int second, Shared& s) {
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const auto least = [](int v) {
+#pragma unroll
+        for (int offset = kWave / 2; offset > 0; offset >>= 1) v = min(v, __shfl_xor(v, offset, kWave));
+        return v;
+    };
+    first = least(first);
+    second = ~least(~second);
+    if (lane == 0) {
+        s.picked[wave] = first;
+        s.last[wave] = second;
+    }
+    __syncthreads();
+    first = least(s.picked[lane % kWaves]);
+    second = ~least(~s.last[lane % kWaves]);
+    __syncthreads();
+    return first != 0x7fffffff ? first : second;
+}
 
 // The place whose running sum passes the target, of thread t's kPlaces from t * kPlaces on (`front` in front of them); the last
 // with any weight if none does, -1 without any.
 __device__ __forceinline__ int pick_place(const u64 (&own)[kPlaces], u64 front, double target, Shared& s) {
-    if (threadIdx.x == 0) {
-        s.picked = 0x7fffffff;
-        s.last = -1;
-    }
-    __syncthreads();
-    int mine = -1, last = -1;
+    int mine = 0x7fffffff, last = -1;
 #pragma unroll
     for (int i = 0; i < kPlaces; ++i) {
         if (own[i] == 0) continue;
         last = threadIdx.x * kPlaces + i;
         front += own[i];
-        if (mine < 0 && static_cast<double>(front) > target) mine = last;
+        if (mine == 0x7fffffff && static_cast<double>(front) > target) mine = last;
     }
-    if (mine >= 0) atomicMin(&s.picked, mine);
-    if (last >= 0) atomicMax(&s.last, last);
-    __syncthreads();
-    return s.picked != 0x7fffffff ? s.picked : s.last;
+    return choose(mine, last, s);
 }
 
 // The draw from one part of the row, of what lies up to `cut` in its order; -1 without any weight.
@@ -678,7 +730,6 @@ __device__ int draw_from_part(const Row& row, Shared& s, int part, u64 before, d
     }
     const u64 front = before + sums_in_front(own, s.sum, total);
     const int place = pick_place(own, front, target, s);
-    __syncthreads();
     return place < 0 ? -1 : part * kPart + place;
 }
 
@@ -714,10 +765,6 @@ __device__ int draw_from_few(const Row& row, Shared& s, int n, const Rules& rule
     if (!kept) weight = 0;
     const double target = u * static_cast<double>(block_sum_u64(lane == 0 ? weight : 0, s.sum));
     if (lane == 0) s.weight[i] = weight;  // (all have read the old ones: the sum has barriers)
-    if (threadIdx.x == 0) {
-        s.picked = 0x7fffffff;
-        s.last = -1;
-    }
     __syncthreads();
     const uint32_t index = static_cast<uint32_t>(mine);
     u64 running = 0;
@@ -725,12 +772,8 @@ __device__ int draw_from_few(const Row& row, Shared& s, int n, const Rules& rule
         if (static_cast<uint32_t>(s.list[j]) <= index) running += s.weight[j];
 #pragma unroll
     for (int offset = 1; offset < 4; offset <<= 1) running += __shfl_xor(running, offset, kWave);
-    if (weight) {
-        if (static_cast<double>(running) > target) atomicMin(&s.picked, static_cast<int>(index));
-        atomicMax(&s.last, static_cast<int>(index));
-    }
-    __syncthreads();
-    return s.picked != 0x7fffffff ? s.picked : s.last;
+    return choose(weight && static_cast<double>(running) > target ? static_cast<int>(index) : 0x7fffffff,
+                  weight ? static_cast<int>(index) : -1, s);
 }
 
 // ... from a longer one.
@@ -744,21 +787,16 @@ __device__ int draw_from_list(const Row& row, Shared& s, int n, const Rules& rul
         own[i] = first + i < n ? row.weight(logit_of(~static_cast<uint32_t>(s.list[first + i] >> 32))) : 0;
     u64 front = sums_in_front(own, s.sum, total);
     const double limit = rules.p * static_cast<double>(total);
-    if (threadIdx.x == 0) s.kept = 0;
-    __syncthreads();
-    int kept = 0;
+    int kept = 0;  // (what is kept is a prefix of all places, so the threads' numbers add up to it)
 #pragma unroll
     for (int i = 0; i < kPlaces; ++i) {
-        if (first + i >= n) break;
-        const float l = logit_of(~static_cast<uint32_t>(s.list[first + i] >> 32));
-        if (first + i > 0 && rules.p < 1.0 && !(static_cast<double>(front) < limit)) break;
-        if (first + i > 0 && rules.m > 0.0 && row.share(l) < rules.m) break;
+        if (first + i >= n) continue;
+        const bool in_p = first + i == 0 || !(rules.p < 1.0) || static_cast<double>(front) < limit;
+        const bool in_m = first + i == 0 || !(rules.m > 0.0) || row.share(logit_of(~static_cast<uint32_t>(s.list[first + i] >> 32))) >= rules.m;
+        kept += in_p && in_m;
         front += own[i];
-        kept = first + i + 1;
     }
-    if (kept) atomicMax(&s.kept, kept);
-    __syncthreads();
-    n = s.kept;
+    n = static_cast<int>(block_sum_u64(kept, s.sum));
     // the kept ones by index, their logits' order beside it
     u64 turned[kPlaces];
 #pragma unroll
@@ -793,7 +831,7 @@ __device__ int draw_of_k(const Row& row, Shared& s, const float* chunks, int chu
         s.h.weight[b] = 0;
         s.h.count[b] = 0;
     }
-    if (threadIdx.x == 0) s.count = s.kept = 0;
+    if (threadIdx.x == 0) s.count = s.hit_count = 0;
     __syncthreads();
     for (int round = 0; round < rounds; ++round) {
         if (round) read(round);
@@ -802,8 +840,8 @@ __device__ int draw_of_k(const Row& row, Shared& s, const float* chunks, int chu
             if (largest[j] > -INFINITY) atomicAdd(&s.h.count[bin_of(largest[j])], 1);
     }
     __syncthreads();
-    cross(s.h, true, rules.k, 0.0);  // (fewer chunks than k: the last bin that has any, and then all below it)
-    const int found = s.h.above_count + s.h.count[s.h.bin] >= rules.k ? s.h.bin : -1;
+    cross<true>(s.h, rules.k, 0.0);  // (fewer chunks than k: the last bin that has any, and then all below it)
+    const int found = s.h.above + s.h.count[s.h.bin] >= static_cast<u64>(rules.k) ? s.h.bin : -1;
     __syncthreads();
     const auto passes = [&](float l) { return l > -INFINITY && bin_of(l) >= found; };
     for (int round = 0; round < rounds; ++round) {
@@ -811,12 +849,12 @@ __device__ int draw_of_k(const Row& row, Shared& s, const float* chunks, int chu
 #pragma unroll
         for (int j = 0; j < kRound; ++j)
             if (passes(largest[j])) {
-                const int at = atomicAdd(&s.kept, 1);
+                const int at = atomicAdd(&s.hit_count, 1);
                 if (at < kList) s.hits[at] = (round * kRound + j) * kThreads + threadIdx.x;
             }
     }
     __syncthreads();
-    const int hits = s.kept;
+    const int hits = s.hit_count;
     if (hits > kList) return -2;  // (each has a number that passes)
     const bool lines = (reinterpret_cast<uintptr_t>(row.logits) & 15) == 0;
     for (int item = threadIdx.x; item < hits * 4; item += kThreads) {
@@ -845,22 +883,33 @@ __device__ int draw_of_k(const Row& row, Shared& s, const float* chunks, int chu
     return n <= kThreads / 4 ? draw_from_few(row, s, n, rules, u) : draw_from_list(row, s, n, rules, u);
 }
 
-// The part in which the running sum of s.segment passes u times the whole, and its draw.
+// The part in which the running sum of s.segment passes u times the whole, and its draw.  (A part whose numbers each round to no
+// weight, though their sum has one, has nothing to draw: the next one then.)
 __device__ int draw_from_segments(const Row& row, Shared& s, int parts, double u, u64 cut) {
-    // (every thread goes through them: a wave would have to tell the others what it found)
+    // every wave the same
+    const int lane = threadIdx.x % kWave;
     u64 all = 0;
-    for (int q = 0; q < parts; ++q) all += s.segment[q];
-    const double target = u * static_cast<double>(all);
+    for (int q = lane; q < parts; q += kWave) all += s.segment[q];
+    const double target = u * static_cast<double>(wave_sum_u64(all));
     int owner = 0;
-    u64 running = 0, before = 0;
-    for (int q = 0; q < parts; ++q) {
-        if (s.segment[q] == 0) continue;
-        owner = q;
-        before = running;
-        running += s.segment[q];
-        if (static_cast<double>(running) > target) break;
+    u64 before = 0, running = 0;
+    for (int base = 0; base < parts; base += kWave) {
+        const u64 own = base + lane < parts ? s.segment[base + lane] : 0;
+        const u64 sum = running + wave_running_u64(own);
+        const u64 passed = __ballot(own && static_cast<double>(sum) > target), any = __ballot(own > 0);
+        if (any) {
+            const int which = passed ? __ffsll(passed) - 1 : 63 - __clzll(any);
+            owner = base + which;
+            const u64 front = sum - own;
+            before = joined(__builtin_amdgcn_readlane(static_cast<int>(front & 0xffffffffu), which),
+                            __builtin_amdgcn_readlane(static_cast<int>(front >> 32), which));
+        }
+        if (passed) break;
+        running = last_lane(sum);
     }
-    return draw_from_part(row, s, owner, before, target, cut);
+    int picked = draw_from_part(row, s, owner, before, target, cut);
+    for (int q = owner + 1; q < parts && picked < 0; ++q) picked = draw_from_part(row, s, q, 0, -1.0, cut);
+    return picked;
 }
 
 // The draw of a row that was tallied; -2: the cut's bin holds more than its list.
@@ -881,21 +930,19 @@ __device__ int draw_of_tally(Row& row, Shared& s, const PartOf& of, int r, int p
         for (int i = 0; i < kPlaces; ++i)
             own[i] = first + i < n ? row.weight(logit_of(~static_cast<uint32_t>(s.list[first + i] >> 32))) : 0;
         u64 front = above + sums_in_front(own, s.sum, weight);
-        if (threadIdx.x == 0) s.kept = 0;
-        __syncthreads();
-        row.least = rules.m;
+        int kept = 0;  // (a prefix of the places)
 #pragma unroll
         for (int i = 0; i < kPlaces; ++i) {
-            if (first + i >= n || !(front == 0 || static_cast<double>(front) < limit)) break;
+            if (first + i >= n || !(front == 0 || static_cast<double>(front) < limit)) continue;
             front += own[i];
-            atomicMax(&s.kept, first + i + 1);
-            const u64 w = row.weight(logit_of(~static_cast<uint32_t>(s.list[first + i] >> 32)));
-            if (w) atomicAdd(&s.segment[static_cast<uint32_t>(s.list[first + i]) / kPart], w);
+            ++kept;
+            const u64 place = s.list[first + i];
+            if (own[i] && (!(rules.m > 0.0) || row.share(logit_of(~static_cast<uint32_t>(place >> 32))) >= rules.m))
+                atomicAdd(&s.segment[static_cast<uint32_t>(place) / kPart], own[i]);
         }
-        __syncthreads();
+        const int last = static_cast<int>(block_sum_u64(kept, s.sum));
         // (nothing of the bin is kept only if rounding says so: the cut then lies right in front of it)
-        cut = s.kept > 0 ? s.list[s.kept - 1] : n > 0 ? s.list[0] - 1 : ~0ull;
-        __syncthreads();
+        cut = last > 0 ? s.list[last - 1] : n > 0 ? s.list[0] - 1 : ~0ull;
     }
     row.least = rules.m;
     return draw_from_segments(row, s, parts, u, cut);
@@ -928,21 +975,10 @@ rules_draw_kernel(const float* __restrict__ logits, const float* __restrict__ te
             __syncthreads();
             picked = draw_of_tally(row, s, of, r, parts, rules, total, u);
         } else {
-            const double target = u * total;
-            int owner = 0;
-            double running = 0.0, before = 0.0;
-            for (int q = 0; q < parts; ++q) {
-                const double mine = s.whole.sum[q];
-                if (mine * unit < 0.5) continue;
-                owner = q;
-                before = running;
-                running += mine;
-                if (running > target) break;
-            }
-            // (a part whose numbers each round to no weight has nothing to draw: the next one then)
-            picked = -1;
-            for (int q = owner; q < parts && picked < 0; ++q)
-                picked = draw_from_part(row, s, q, 0, q == owner ? (target - before) * unit : -1.0, ~0ull);
+            __syncthreads();
+            for (int q = threadIdx.x; q < parts; q += kThreads) s.segment[q] = static_cast<u64>(s.whole.sum[q] * unit + 0.5);
+            __syncthreads();
+            picked = draw_from_segments(row, s, parts, u, ~0ull);
         }
     }
     if (picked == -2) {
