@@ -1537,20 +1537,29 @@ def _sample_rules(logits, temperature, uniform, out, top_k, top_p, min_p) -> tor
     return out
 
 
+# What a workgroup takes of a row at a time, and the workgroups (of 256 threads) that fill the GPU: a row is cut in parts for these
+LOGPROB_TURN, LOGPROB_SPREAD = 4096, 2048
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """What the rows of float32 logits give their tokens (int32 [rows]): ``(l_t - max l) - log sum_i exp(l_i - max l)``, float32
     [rows].  The rows of ``logits`` may lie apart.  A token outside the vocabulary gives NaN, and so does a row with a NaN, a
     +inf, or nothing but -inf."""
     rows, vocab = _logit_rows(logits)
     _per_row("tokens", tokens, torch.int32, rows)
+    if rows > MAX_RULE_ROWS or vocab > 1 << 30:
+        raise ValueError(f"up to {MAX_RULE_ROWS} rows of {1 << 30} logits, not {rows} of {vocab}")
     if out is None:
         out = torch.empty((rows,), dtype=torch.float32, device=logits.device)
     _per_row("out", out, torch.float32, rows)
     _on_current_gpu(logits, tokens, out)
     if rows == 0:
         return out
-    _run("cie_token_logprobs", load_library().cie_token_logprobs(_stream(), _ptr(logits), _ptr(tokens), _ptr(out), _i(rows),
-                                                                _i(vocab), _i(_ld(logits))))
+    turns = -(-vocab // LOGPROB_TURN)
+    part = -(-turns // min(turns, max(1, LOGPROB_SPREAD // rows))) * LOGPROB_TURN
+    tallies = None if part >= vocab else torch.empty(2 * rows * -(-vocab // part), dtype=torch.float32, device=logits.device)
+    _run("cie_token_logprobs", load_library().cie_token_logprobs(
+        _stream(), _ptr(logits), _ptr(tokens), _ptr(tallies), _ptr(out), _i(rows), _i(vocab), _i(_ld(logits)), _i(part)))
     return out
 
 
