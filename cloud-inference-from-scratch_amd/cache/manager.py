@@ -310,9 +310,11 @@ class CacheManager:
         return fresh
 
     # -- admission ------------------------------------------------------------
-    def admit(self, request_id: str, prompt_tokens: Sequence[int] | None = None) -> int:
+    def admit(self, request_id: str, prompt_tokens: Sequence[int] | None = None, variant: int | None = None) -> int:
         """Give the request a slot and empty tables; returns how many leading
-        prompt tokens are already cached (taken over from the prefix index)."""
+        prompt tokens are already cached (taken over from the prefix index).  ``variant``: the request
+        runs the model in a form of its own (an adapter beside its weights), whose keys and values are
+        no other form's: it shares pages with requests of the same variant only."""
         if request_id in self._slots:
             raise ValueError(f"duplicate admission of {request_id}")
         if request_id == PREFIX_HOLDER:
@@ -328,7 +330,7 @@ class CacheManager:
             group.tables[request_id] = []
             self._dirty.add((index, slot))
         if prompt_tokens is not None and self.prefix_cache_pages:
-            return self._restore_prefix(request_id, prompt_tokens)
+            return self._restore_prefix(request_id, prompt_tokens, variant)
         return 0
 
     # -- growth ---------------------------------------------------------------
@@ -384,13 +386,13 @@ class CacheManager:
                     self._dirty.add((index, self._slots[request_id]))
 
     # -- release --------------------------------------------------------------
-    def release(self, request_id: str, prompt_tokens: Sequence[int] | None = None) -> None:
+    def release(self, request_id: str, prompt_tokens: Sequence[int] | None = None, variant: int | None = None) -> None:
         """Give back the request's slot and pages.  With ``prompt_tokens`` its full
         prompt pages are first offered to the prefix index (not on preemption)."""
         if request_id not in self._slots:
             return
         if prompt_tokens is not None and self.prefix_cache_pages:
-            self._store_prefix(request_id, prompt_tokens)
+            self._store_prefix(request_id, prompt_tokens, variant)
         slot = self._slots.pop(request_id)
         for index, group in enumerate(self.groups):
             table = group.tables.pop(request_id)
@@ -402,18 +404,23 @@ class CacheManager:
         self._free_slots.append(slot)
 
     # -- prefix index -----------------------------------------------------------
-    def publish_prefix(self, request_id: str, prompt_tokens: Sequence[int]) -> int:
+    def publish_prefix(self, request_id: str, prompt_tokens: Sequence[int], variant: int | None = None) -> int:
         """Offer the full prompt pages a live request has committed to the prefix index; the request
         keeps them (a page then has two holders and is read-only for both).  Returns the tokens indexed."""
         if request_id not in self._slots or not self.prefix_cache_pages:
             return 0
-        return self._store_prefix(request_id, prompt_tokens)
+        return self._store_prefix(request_id, prompt_tokens, variant)
 
-    def _restore_prefix(self, request_id: str, tokens: Sequence[int]) -> int:
+    @staticmethod
+    def _root(variant: int | None) -> tuple | None:
+        """What stands in a first page's key where later ones have the page above."""
+        return None if variant is None else ("variant", variant)
+
+    def _restore_prefix(self, request_id: str, tokens: Sequence[int], variant: int | None = None) -> int:
         group = self.groups[0]
         candidate_pages = (len(tokens) - 1) // self.page_size
         matched: list[_PrefixNode] = []
-        parent_id: int | None = None
+        parent_id = self._root(variant)
         size, find = self.page_size, self._prefix.get
         for first in range(0, candidate_pages * size, size):
             node = find((parent_id, tuple(tokens[first:first + size])))
@@ -437,14 +444,14 @@ class CacheManager:
         self.prefix_cache_hits += 1
         return length
 
-    def _store_prefix(self, request_id: str, tokens: Sequence[int]) -> int:
+    def _store_prefix(self, request_id: str, tokens: Sequence[int], variant: int | None = None) -> int:
         group = self.groups[0]
         table = group.tables[request_id]
         pages = min((len(tokens) - 1) // self.page_size, self._length[request_id] // self.page_size, len(table))
         parent: _PrefixNode | None = None
         stored = 0
         for i in range(pages):
-            key = (parent.serial if parent is not None else None,
+            key = (parent.serial if parent is not None else self._root(variant),
                    tuple(tokens[i * self.page_size:(i + 1) * self.page_size]))
             node = self._prefix.get(key)
             if node is None:

@@ -49,6 +49,11 @@ def parser() -> argparse.ArgumentParser:
     generate.add_argument("--token-ids", help="comma or space separated prompt token ids")
     generate.add_argument("--max-output-tokens", type=int, default=64)
     generate.add_argument("--temperature", type=float, default=0.0)
+    generate.add_argument("--top-k", type=int, default=0, help="draw from the K likeliest tokens only (0: all)")
+    generate.add_argument("--top-p", type=float, default=1.0, help="... from the likeliest that make up this share (1: all)")
+    generate.add_argument("--min-p", type=float, default=0.0, help="... from those at least this likely, relative to the likeliest")
+    generate.add_argument("--logprobs", action="store_true", help="print the tokens' log-probabilities as JSON afterwards")
+    generate.add_argument("--adapter", metavar="DIR", help="a low-rank adapter's folder (adapter_config.json + adapter_model.safetensors)")
     generate.add_argument("--ignore-eos", action="store_true")
     generate.add_argument("--no-stream", action="store_true")
     generate.add_argument("--metrics", action="store_true", help="print the run's metrics as JSON afterwards")
@@ -86,6 +91,10 @@ def _make_engine(args: argparse.Namespace):
             options[name] = getattr(args, name)
     if args.kv_pages is not None:
         options["kv_tokens"] = args.kv_pages * options.get("page_size", EngineConfig.page_size)
+    adapter = getattr(args, "adapter", None)
+    if adapter:
+        with open(Path(adapter) / "adapter_config.json", encoding="utf-8") as handle:
+            options.update(max_adapters=1, max_adapter_rank=int(json.load(handle).get("r", EngineConfig.max_adapter_rank)))
     if args.random_weights:
         with open(args.random_weights, encoding="utf-8") as handle:
             config = config_from_dict(json.load(handle))
@@ -158,8 +167,11 @@ def main(argv: list[str] | None = None) -> int:
     else:
         raise SystemExit("cie generate: give PROMPT or --token-ids")
     eos = None if args.ignore_eos else getattr(engine.model_config, "eos_token_id", None)
+    if args.adapter:
+        engine.load_adapter("adapter", args.adapter)
     gen = GenerationConfig(max_output_tokens=args.max_output_tokens, temperature=args.temperature,
-                           eos_token_id=eos, seed=args.seed if args.temperature > 0 else None)
+                           eos_token_id=eos, seed=args.seed if args.temperature > 0 else None, top_k=args.top_k, top_p=args.top_p,
+                           min_p=args.min_p, logprobs=args.logprobs, adapter="adapter" if args.adapter else None)
     as_text = isinstance(prompt, str)
     streaming = not args.no_stream
 
@@ -172,6 +184,8 @@ def main(argv: list[str] | None = None) -> int:
         print()
     else:
         print(result.text if as_text else " ".join(map(str, result.token_ids)))
+    if args.logprobs:
+        print(json.dumps({"logprobs": result.logprobs}))
     if args.metrics:
         print(json.dumps(engine.snapshot_metrics(), indent=2))
     return 0

@@ -57,6 +57,10 @@ class EngineConfig:
     # algorithm the vendor library has for their shapes at their first call, a few seconds each, instead of
     # the handful its heuristic proposes; False: the heuristic's candidates only
     search_library_algorithms: bool = True
+    # low-rank adapters that can be loaded beside the weights at a time (their memory is set aside at the start), and the
+    # largest rank they may have
+    max_adapters: int = 0
+    max_adapter_rank: int = 16
     seed: int = 0
 
     def validated(self) -> "EngineConfig":
@@ -71,6 +75,10 @@ class EngineConfig:
             raise ValueError("prefix_cache_pages must be non-negative")
         if config.graph_mixed_steps < 0:
             raise ValueError("graph_mixed_steps must be non-negative")
+        if config.max_adapters < 0:
+            raise ValueError("max_adapters must be non-negative")
+        if not 1 <= config.max_adapter_rank <= 128:
+            raise ValueError("max_adapter_rank must lie between 1 and 128")
         if config.kv_tokens is not None and config.kv_tokens < config.page_size:
             raise ValueError("kv_tokens too small for even one page")
         if config.kv_cache_bytes is not None and config.kv_cache_bytes < 1:

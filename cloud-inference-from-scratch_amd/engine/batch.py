@@ -56,6 +56,8 @@ class StepBatch:
     token_pool: Any = None
     # a captured decode step: where the address of the logits' matrix lies (int64 [1] on the device), which every replay may change
     logits_at: Any = None
+    # low-rank adapters: int32 [T] on the device, the slot of each row's adapter (< 0: none); None: no row of the step has one
+    adapters: Any = None
     # what one layer of a step hands to later ones (the model empties it at the step's start): tensors by name
     carried: dict = field(default_factory=dict)
     _tiles: dict = field(default_factory=dict)

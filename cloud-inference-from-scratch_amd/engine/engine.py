@@ -17,6 +17,8 @@ from typing import Any
 
 from ..config.engine_config import EngineConfig, build_engine_config
 from ..metrics import Metrics
+from .adapters import Adapters, read_adapter
+from ..parts.adapters import AdapterRoom
 from .loading import load_model, random_model
 from .runner import Runner
 from .plan import decodes_before_prompts, most_resident_gives_way
@@ -34,6 +36,7 @@ class GenerationResult:
     finish_reason: str
     ttft_ms: float | None
     e2e_ms: float
+    logprobs: list[float] | None = None  # one for each of ``token_ids``, where the request asked for them
 
 
 class Engine:
@@ -50,6 +53,7 @@ class Engine:
         self.engine_config = build_engine_config(engine_config, **options)
         self.model_dir = Path(model_dir) if model_dir is not None else None
         self.tokenizer = None
+        self.adapters: Adapters | None = None
         if runner_factory is not None:
             self.model = None
             self.model_config = config
@@ -66,6 +70,8 @@ class Engine:
             positions = self.model.spec.max_position
             if self.engine_config.max_model_len > positions:
                 self.engine_config = build_engine_config(self.engine_config, max_model_len=positions)
+            if self.engine_config.max_adapters:  # (before the cache takes its share of the memory that is free)
+                self.adapters = Adapters(AdapterRoom(self.model, self.engine_config.max_adapters, self.engine_config.max_adapter_rank))
             self.runner = Runner(self.model, self.engine_config, device)
         self.metrics = Metrics()
         self.scheduler = Scheduler(self.engine_config, self.runner, self.metrics,
@@ -103,7 +109,30 @@ class Engine:
                on_token: Callable[[Request, int], None] | None = None) -> Request:
         token_ids = self.tokenize(prompt) if isinstance(prompt, str) else list(prompt)
         label = prompt if isinstance(prompt, str) else ""
-        return self.scheduler.submit(token_ids, self._generation_config(gen), label=label, on_token=on_token)
+        config = self._generation_config(gen)
+        adapter = self._adapters().find(config.adapter) if config.adapter is not None else None
+        return self.scheduler.submit(token_ids, config, label=label, on_token=on_token, adapter=adapter)
+
+    # -- low-rank adapters ---------------------------------------------------------------
+    def _adapters(self) -> Adapters:
+        if self.adapters is None:
+            raise ValueError("this engine was made without room for adapters (max_adapters)")
+        return self.adapters
+
+    def load_adapter(self, name: str, folder: str | Path | None = None, *, tensors: Any = None, scale: float | None = None) -> None:
+        """Load a low-rank adapter beside the weights, for requests whose ``GenerationConfig.adapter`` names it: a folder
+        with ``adapter_config.json`` and ``adapter_model.safetensors``, or ``tensors`` (``<projection>.lora_A.weight`` [r, in] and
+        ``<projection>.lora_B.weight`` [out, r]) and the ``scale`` of their product.  It takes one of ``max_adapters`` slots."""
+        adapters = self._adapters()
+        if (folder is None) == (tensors is None) or (tensors is None) != (scale is None):
+            raise ValueError("give an adapter's folder, or its tensors and their scale")
+        if folder is not None:
+            tensors, scale = read_adapter(folder)
+        adapters.load(name, tensors, float(scale))
+
+    def unload_adapter(self, name: str) -> None:
+        """Free the adapter's slot; refused while a request that has it is not finished."""
+        self._adapters().unload(name, [*self.scheduler.active, *self.scheduler.waiting])
 
     def step(self) -> bool:
         return self.scheduler.step()
@@ -130,6 +159,7 @@ class Engine:
             finish_reason=request.finish_reason,
             ttft_ms=(request.first_token_ns - request.arrived_ns) / 1e6 if request.first_token_ns else None,
             e2e_ms=(end - request.arrived_ns) / 1e6,
+            logprobs=list(request.logprobs) if request.gen.logprobs else None,
         )
 
     def generate(self, prompts: Sequence[str | Sequence[int]],

@@ -56,8 +56,10 @@ def _collector_off() -> Iterator[None]:
 
 class _Bucket:
     def __init__(self, size: int, device: torch.device, pad_slot: int, max_keys: int,
-                 token_pool: torch.Tensor | None = None) -> None:
+                 token_pool: torch.Tensor | None = None, adapted: bool = False) -> None:
         self.size = size
+        # a bucket for steps in which some rows have a low-rank adapter: each row's slot, -1 where it has none
+        self.adapters = torch.full((size,), -1, dtype=torch.int32, device=device) if adapted else None
         count = 11 * size + 2
         count += count % 2 + 2  # (behind them, on 8 bytes, the address of the logits)
         self.host = torch.zeros(count, dtype=torch.int32)  # the template; every replay stages a copy of it
@@ -97,7 +99,7 @@ class _Bucket:
             host_slots=[pad_slot] * size, host_starts=[0] * size, host_q_lens=[1] * size,
             static_plan=StaticPlan(view("tile_seq"), view("tile_q0"), view("max_context", 1), max_keys),
             token_feed=view("token_feed") if token_pool is not None else None, token_pool=token_pool,
-            logits_at=view("logits_at", 2).view(torch.int64),
+            logits_at=view("logits_at", 2).view(torch.int64), adapters=self.adapters,
         )
         # what a replay rewrites, for the kernel that does (its arguments carry the numbers: a pinned buffer, a copy into it and
         # one to the device were 14 us of the host's 75 a step of the smallest model, and 3.6 against 2 us of the GPU's)
@@ -134,6 +136,7 @@ class DecodeGraphs:
         self.runner = runner
         self.largest = largest or 1 << (max(runner.config.max_running, 1) - 1).bit_length()
         self.buckets: dict[int, _Bucket] = {}
+        self.adapted_buckets: dict[int, _Bucket] = {}  # for steps in which some rows have a low-rank adapter
         # the tokens the last step sampled, on the device: a step may start from them before the host has them
         self.token_pool = torch.zeros(self.largest, dtype=torch.int32, device=runner.device)
         self.pool: Any = None
@@ -147,10 +150,10 @@ class DecodeGraphs:
     def bucket_of(sequences: int) -> int:
         return 1 << (sequences - 1).bit_length()
 
-    def _capture(self, size: int) -> _Bucket:
+    def _capture(self, size: int, adapted: bool = False) -> _Bucket:
         runner = self.runner
         bucket = _Bucket(size, runner.device, runner.device_cache.pad_slot, runner.config.max_model_len,
-                         self.token_pool)
+                         self.token_pool, adapted)
         logits = self._logits(size)  # (of the run on padding)
         bucket.fill([], [], [], 1, logits=logits)
         bucket.dev.copy_(bucket.host)
@@ -168,9 +171,12 @@ class DecodeGraphs:
         with _collector_off(), torch.cuda.graph(graph, pool=self.pool):
             bucket.logits = runner.model.forward(bucket.batch, runner.device_cache)
         bucket.graph = graph
-        self.buckets[size] = bucket
+        self._buckets(adapted)[size] = bucket
         self.captures += 1
         return bucket
+
+    def _buckets(self, adapted: bool) -> dict[int, _Bucket]:
+        return self.adapted_buckets if adapted else self.buckets
 
     def _logits(self, size: int) -> torch.Tensor:
         return torch.empty((size, self.runner.model.head.shape[0]), dtype=torch.float32, device=self.runner.device)
@@ -181,9 +187,10 @@ class DecodeGraphs:
         made = 0
         size = 1
         while size <= self.largest:
-            if size not in self.buckets:
-                self._capture(size)
-                made += 1
+            for adapted in (False, True) if self.runner.adapter_slots else (False,):
+                if size not in self._buckets(adapted):
+                    self._capture(size, adapted)
+                    made += 1
             size *= 2
         return made
 
@@ -197,7 +204,8 @@ class DecodeGraphs:
         the next replay can start)."""
         runner = self.runner
         size = self.bucket_of(len(entries))
-        bucket = self.buckets.get(size) or self._capture(size)
+        adapted = any(e.adapter >= 0 for e in entries)
+        bucket = self._buckets(adapted).get(size) or self._capture(size, adapted)
         cache = runner.cache
         positions = [e.start_pos for e in entries]
         tokens, slots = [e.tokens[0] for e in entries], [cache.slot(e.request_id) for e in entries]
@@ -211,6 +219,9 @@ class DecodeGraphs:
         else:
             bucket.fill(tokens, positions, slots, max(positions) + 1, feed, logits)
             bucket.dev.copy_(to_device_staging(bucket.host, runner.device), non_blocking=True)
+        if adapted:
+            slots_of = [e.adapter for e in entries] + [-1] * (size - len(entries))
+            bucket.adapters.copy_(to_device_staging(slots_of, runner.device), non_blocking=True)
         bucket.graph.replay()
         self.replays += 1
         rows = [index for index, e in enumerate(entries) for _ in e.want]
@@ -283,6 +294,8 @@ class MixedGraphs:
                 return None
         if any(len(e.want) > 1 for e in single):
             return None
+        if any(e.adapter >= 0 for e in entries):
+            return None  # (steps of portions in which rows have adapters run launch by launch)
         return bucket, tuple(len(e.tokens) for e in portions)
 
     def wants(self, entries: Sequence[Any]) -> tuple | None:

@@ -13,6 +13,7 @@ from __future__ import annotations
 from collections.abc import Callable
 from dataclasses import dataclass, field
 from enum import Enum
+from typing import Any
 
 
 class RequestState(Enum):
@@ -51,18 +52,53 @@ class GenerationConfig:
     offers (src/cloud_engine/scheduler.py:63-71); a positive temperature draws
     from softmax(logits / temperature) with a random number that depends on
     ``seed`` and the token's index only, never on the batch.  Without an
-    ``eos_token_id`` only ``max_output_tokens`` ends the request."""
+    ``eos_token_id`` only ``max_output_tokens`` ends the request.
+
+    ``top_k`` (0: off), ``top_p`` (1: off) and ``min_p`` (0: off) are the rules that a draw
+    with a temperature is under (``ops.sample``).  ``logprobs``: the result brings what the
+    model itself, without temperature and rules, gave each token it produced.  ``adapter``: the
+    name of a low-rank adapter that the engine has loaded."""
 
     max_output_tokens: int
     temperature: float = 0.0
     eos_token_id: int | None = None
     seed: int | None = None
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+    logprobs: bool = False
+    adapter: str | None = None
 
     def __post_init__(self) -> None:
         if self.max_output_tokens < 1:
             raise ValueError("max_output_tokens must be positive")
         if not self.temperature >= 0:
             raise ValueError("temperature must be zero (greedy) or positive")
+        if not 0 <= self.top_k < 1 << 31 or int(self.top_k) != self.top_k:
+            raise ValueError("top_k must be zero (off) or a positive whole number")
+        if not 0 < self.top_p <= 1:
+            raise ValueError("top_p must lie in (0, 1]")
+        if not 0 <= self.min_p <= 1:
+            raise ValueError("min_p must lie in [0, 1]")
+
+    @property
+    def rules(self) -> tuple[int, float, float] | None:
+        """(top_k, top_p, min_p) where the request draws under any of them."""
+        if self.temperature > 0 and (self.top_k > 0 or self.top_p < 1 or self.min_p > 0):
+            return int(self.top_k), self.top_p, self.min_p
+        return None
+
+
+class ScoredToken(int):
+    """A sampled token that brings its log-probability."""
+
+    logprob: float
+
+    @classmethod
+    def of(cls, token: int, logprob: float) -> "ScoredToken":
+        made = cls(token)
+        made.logprob = logprob
+        return made
 
 
 @dataclass
@@ -76,6 +112,8 @@ class Request:
     on_token: Callable[["Request", int], None] | None = None
     state: RequestState = RequestState.WAITING
     output: list[int] = field(default_factory=list)
+    logprobs: list[float] = field(default_factory=list)  # of the output's tokens, where the request asks for them
+    adapter: Any = None         # what the engine knows of the adapter the request has (``slot``, ``serial``)
     cached: int = 0             # tokens of prompt + output that the cache holds (the runner moves it)
     first_token_ns: int | None = None
     latest_token_ns: int | None = None

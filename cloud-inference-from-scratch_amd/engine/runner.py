@@ -29,6 +29,7 @@ from ..sampling.sampler import Sampler
 from .batch import StepBatch
 from .device_cache import DeviceCache
 from .graphs import DecodeGraphs, MixedGraphs
+from .request import ScoredToken
 
 
 @dataclass(frozen=True)
@@ -41,6 +42,7 @@ class StepEntry:
     tokens: Sequence[int]
     start_pos: int
     want: Sequence[int] = field(default_factory=tuple)
+    adapter: int = -1  # the slot of the low-rank adapter that the request has
 
 
 @dataclass
@@ -50,10 +52,16 @@ class PendingTokens:
     request_ids: tuple[str, ...]
     host: torch.Tensor          # page-locked int32 [n]; valid once ``ready`` has passed
     ready: Any                  # torch.cuda.Event behind the copy
+    scores: torch.Tensor | None = None  # their log-probabilities likewise (float32 [n]), where a request asks for them
 
     def tokens(self) -> dict[str, int]:
         self.ready.synchronize()
-        return dict(zip(self.request_ids, self.host.tolist()))
+        return dict(zip(self.request_ids, scored(self.host.tolist(), self.scores)))
+
+
+def scored(tokens: list[int], scores: torch.Tensor | None) -> list[int]:
+    """The tokens, with their log-probabilities if there are any (in host memory)."""
+    return tokens if scores is None else [ScoredToken.of(*both) for both in zip(tokens, scores.tolist())]
 
 
 # What a running engine needs of the device memory beside weights and cache, set aside before the cache takes
@@ -63,6 +71,14 @@ class PendingTokens:
 # projections and feed-forward, and partial sums, some 64 bytes) and float32 logits.
 LIBRARY_TIMING_BYTES = 640 << 20
 ACTIVATION_BYTES_PER_NUMBER = 64
+
+
+def _slot_of_adapter(request: Any) -> int:
+    return -1 if request.adapter is None else request.adapter.slot
+
+
+def _variant(request: Any) -> int | None:
+    return None if request.adapter is None else request.adapter.serial
 
 
 def flat_needs(needs: Sequence[Any]) -> list[Any]:
@@ -142,10 +158,10 @@ class Runner:
 
     # -- what the scheduler calls ------------------------------------------------
     def admit(self, request: Any) -> None:
-        request.cached = self.cache.admit(request.request_id, request.prompt)
+        request.cached = self.cache.admit(request.request_id, request.prompt, _variant(request))
 
     def release(self, request: Any, preempted: bool = False) -> None:
-        self.cache.release(request.request_id, None if preempted else request.prompt)
+        self.cache.release(request.request_id, None if preempted else request.prompt, _variant(request))
 
     def warm_up(self) -> int:
         """Do now what the first steps would otherwise do on the clock: capture the decode graphs of
@@ -164,7 +180,7 @@ class Runner:
     def publish_prefix(self, request: Any) -> None:
         """The request's prompt is in the cache: offer its full pages to the prefix index now, not only
         when it ends (the reference stores at release, src/cloud_engine/engine.py:224-226)."""
-        self.cache.publish_prefix(request.request_id, request.prompt)
+        self.cache.publish_prefix(request.request_id, request.prompt, _variant(request))
 
     def allocated_tokens(self, request: Any) -> int:
         return self.cache.allocated_tokens(request.request_id)
@@ -200,7 +216,7 @@ class Runner:
         ``execute_batch``, src/cloud_engine/engine.py:439-488)."""
         entries = [
             StepEntry(portion.request.request_id, portion.tokens, portion.start,
-                      (portion.length - 1,) if portion.samples else ())
+                      (portion.length - 1,) if portion.samples else (), _slot_of_adapter(portion.request))
             for portion in plan.portions
         ]
         logits = self.run(entries, borrow_logits=True)  # (sampled from at once, below)
@@ -210,12 +226,15 @@ class Runner:
         if not sampling:
             return {}
         with trace_range("ragged.sample"):
-            tokens = self.sampler.sample(
+            on_device = self.sampler.sample_on_device(
                 logits,
                 [r.gen.temperature for r in sampling],
                 [self.sampler.uniform(r.gen.seed, r.serial, len(r.output)) if r.gen.temperature > 0 else 0.0
                  for r in sampling],
+                rules=[r.gen.rules for r in sampling],
             )
+            scores = ops.token_logprobs(logits, on_device) if any(r.gen.logprobs for r in sampling) else None
+            tokens = scored(on_device.tolist(), None if scores is None else scores.cpu())
         return {r.request_id: token for r, token in zip(sampling, tokens)}
 
     # -- decode steps that do not wait for their tokens -----------------------------------
@@ -232,7 +251,7 @@ class Runner:
         on the device for the next launch and travel to the host behind the step;
         :meth:`PendingTokens.tokens` waits for them."""
         assert self.graphs is not None and all(p.length == 1 and p.samples for p in plan.portions)
-        entries = [StepEntry(p.request.request_id, p.tokens, p.start, (0,)) for p in plan.portions]
+        entries = [StepEntry(p.request.request_id, p.tokens, p.start, (0,), _slot_of_adapter(p.request)) for p in plan.portions]
         logits = self.run(entries, feed=feed, borrow_logits=True)
         requests = [p.request for p in plan.portions]
         for p in plan.portions:
@@ -243,12 +262,21 @@ class Runner:
                 logits, [r.gen.temperature for r in requests],
                 [self.sampler.uniform(r.gen.seed, r.serial, index) if r.gen.temperature > 0 else 0.0
                  for r, index in zip(requests, token_indices)],
-                out=pool)
+                out=pool, rules=[r.gen.rules for r in requests])
             host = torch.empty(len(requests), dtype=torch.int32, pin_memory=True)
             host.copy_(pool, non_blocking=True)
+            scores = None
+            if any(r.gen.logprobs for r in requests):
+                scores = torch.empty(len(requests), dtype=torch.float32, pin_memory=True)
+                scores.copy_(ops.token_logprobs(logits, pool), non_blocking=True)
             ready = torch.cuda.Event()
             ready.record()
-        return PendingTokens(tuple(r.request_id for r in requests), host, ready)
+        return PendingTokens(tuple(r.request_id for r in requests), host, ready, scores)
+
+    @property
+    def adapter_slots(self) -> int:
+        room = getattr(self.model, "adapter_room", None)
+        return 0 if room is None else room.count
 
     # -- packing -----------------------------------------------------------------
     def _stage(self, count: int) -> torch.Tensor:
@@ -275,6 +303,8 @@ class Runner:
             count = len(entry.tokens)
             if count == 0:
                 raise ValueError(f"request {entry.request_id} brings no tokens")
+            if entry.adapter >= self.adapter_slots:
+                raise ValueError(f"request {entry.request_id} has adapter {entry.adapter} of {self.adapter_slots}")
             held = self.cache.length(entry.request_id)
             if entry.start_pos != held:
                 raise ValueError(
@@ -300,7 +330,8 @@ class Runner:
         for count in count_of:
             q_start_loc.append(q_start_loc[-1] + count)
         logit_rows = [q_start_loc[index] + place for index, entry in enumerate(entries) for place in entry.want]
-        sizes = [total, total, total, sequences, sequences, sequences, sequences + 1, len(logit_rows)]
+        adapted = any(entry.adapter >= 0 for entry in entries)
+        sizes = [total, total, total, sequences, sequences, sequences, sequences + 1, len(logit_rows), total if adapted else 0]
         staged = torch.empty(sum(sizes), dtype=torch.int32, pin_memory=self.device.type == "cuda")
         host = staged.numpy()
         bounds = [0]
@@ -319,6 +350,8 @@ class Runner:
         part[5][:] = count_of
         part[6][:] = q_start_loc
         part[7][:] = logit_rows
+        if adapted:
+            part[8][:] = np.repeat(np.asarray([entry.adapter for entry in entries], dtype=np.int32), counts)
         dev = self._stage(staged.numel())
         dev[: staged.numel()].copy_(staged, non_blocking=True)
         views = [dev[bounds[i]: bounds[i + 1]] for i in range(len(sizes))]
@@ -327,6 +360,7 @@ class Runner:
             seq_of_token=views[2], seq_slot=views[3], seq_start=views[4], seq_q_len=views[5],
             q_start_loc=views[6], logit_rows=views[7], host_slots=slots, host_starts=starts,
             host_q_lens=count_of, request_ids=tuple(e.request_id for e in entries),
+            adapters=views[8] if adapted else None,
         )
 
     # -- the step ------------------------------------------------------------------

@@ -96,7 +96,7 @@ class Scheduler:
 
     # ---------------------------------------------------------------- callers
     def submit(self, prompt: Sequence[int], gen: GenerationConfig, label: str = "",
-               on_token: Callable[[Request, int], None] | None = None) -> Request:
+               on_token: Callable[[Request, int], None] | None = None, adapter: Any = None) -> Request:
         """Queue a request, or refuse it (src/cloud_engine/scheduler.py:233-254): no
         prompt, prompt + output beyond ``max_model_len``, queue full."""
         limits = self.config
@@ -109,7 +109,7 @@ class Scheduler:
         self._submitted += 1
         serial = self._submitted
         request = Request(request_id="req-%08d" % serial, serial=serial, prompt=tuple(int(t) for t in prompt),
-                          gen=gen, arrived_ns=self.clock(), label=label, on_token=on_token)
+                          gen=gen, arrived_ns=self.clock(), label=label, on_token=on_token, adapter=adapter)
         self.waiting.append(request)
         return request
 
@@ -254,7 +254,10 @@ class Scheduler:
             if not portion.samples:
                 request.state = RequestState.PREFILL
             elif request.request_id in sampled:
-                self._token_arrived(request, int(sampled[request.request_id]), now)
+                token = sampled[request.request_id]
+                if request.gen.logprobs:
+                    request.logprobs.append(getattr(token, "logprob", float("nan")))
+                self._token_arrived(request, int(token), now)
             else:
                 self._retire(request, RequestState.FAILED, "failed", error="packed runner omitted sampled token")
         self.metrics.iteration(len(plan.portions), plan.token_count)

@@ -23,6 +23,7 @@ from ..cache.manager import PagedKV
 from ..config.specs import PartSpec
 from ..kernels import ops
 from ..weights.tensors import TensorSpec
+from .adapters import Module, Site, add_behind, rows_complete
 from .base import Part, build_part, register_part
 from .linear import Added, BEHIND_ROTATION, FUSED_ROWS, FUSED_SMALL_ROWS, FUSED_SMALL_WEIGHT, RawRows, choose_tiles, cuts_k, linear, takes_tiles
 
@@ -34,6 +35,7 @@ class Attention(Part):
     takes_raw_rows = True  # its first product can make the norm of a few rows itself
     sums_parts = True  # its last product may come back as parts of K
     adds_unordered = True  # ... or merge a decode step's shares itself, and add their sums to the stream in no fixed order
+    takes_adapters = True  # rows of a step may each have a low-rank adapter beside its products
     def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: int, head_dim: int,
                  qkv_bias: bool, out_bias: bool, position: PartSpec, window: Optional[int] = None,
                  scale: Optional[float] = None) -> None:
@@ -84,17 +86,7 @@ class Attention(Part):
     def bind(self, tensors, prefix, dtype, device) -> None:
         super().bind(tensors, prefix, dtype, device)
         names = ("q_proj", "k_proj", "v_proj")
-        extra = self.kernel_head_dim - self.head_dim
-
-        def per_head(t: torch.Tensor) -> torch.Tensor:
-            # [heads * head_dim, ...] -> [heads * kernel_head_dim, ...], each head followed by zero rows
-            if not extra:
-                return t
-            heads = t.shape[0] // self.head_dim
-            padded = t.new_zeros((heads, self.kernel_head_dim) + tuple(t.shape[1:]))
-            padded[:, : self.head_dim] = t.reshape((heads, self.head_dim) + tuple(t.shape[1:]))
-            return padded.reshape((heads * self.kernel_head_dim,) + tuple(t.shape[1:]))
-
+        per_head = self._per_head
         self.w_qkv = torch.cat([per_head(tensors[f"{prefix}{n}.weight"]) for n in names], dim=0).contiguous()
         self.b_qkv = (
             torch.cat([per_head(tensors[f"{prefix}{n}.bias"]) for n in names], dim=0).contiguous()
@@ -104,6 +96,26 @@ class Attention(Part):
         self.cuts_o = cuts_k(*self.w_o.shape)  # (whose sum has no fixed order then, whoever merges its rows)
         self.b_o = tensors[prefix + "o_proj.bias"].contiguous() if self.out_bias else None
         self.cos, self.sin = self.position.tables(device)
+
+    def _per_head(self, t: torch.Tensor) -> torch.Tensor:
+        # [heads * head_dim, ...] -> [heads * kernel_head_dim, ...], each head followed by zero rows
+        if self.kernel_head_dim == self.head_dim:
+            return t
+        heads = t.shape[0] // self.head_dim
+        padded = t.new_zeros((heads, self.kernel_head_dim) + tuple(t.shape[1:]))
+        padded[:, : self.head_dim] = t.reshape((heads, self.head_dim) + tuple(t.shape[1:]))
+        return padded.reshape((heads * self.kernel_head_dim,) + tuple(t.shape[1:]))
+
+    def make_sites(self, count: int, rank: int, scale: torch.Tensor) -> dict[str, Module]:
+        """Room for adapters beside the two products, by the names of the checkpoint's projections."""
+        heads, wide = (self.num_heads, self.num_kv_heads, self.num_kv_heads), self.kernel_head_dim
+        self.site_qkv = Site(self.hidden_size, [h * wide for h in heads], count, rank, self.dtype, self.device, scale)
+        self.site_o = Site(self.num_heads * wide, [self.hidden_size], count, rank, self.dtype, self.device, scale)
+        out = {name: Module(self.site_qkv, piece, self.hidden_size, heads[piece] * self.head_dim, shape_b=self._per_head)
+               for piece, name in enumerate(("q_proj", "k_proj", "v_proj"))}
+        out["o_proj"] = Module(self.site_o, 0, self.num_heads * self.head_dim, self.hidden_size,
+                               shape_a=lambda a: self._per_head(a.t()).t())
+        return out
 
     def warm_up(self, rows: int) -> None:
         blank = lambda width: torch.zeros((rows, width), dtype=self.w_qkv.dtype, device=self.w_qkv.device)
@@ -124,6 +136,8 @@ class Attention(Part):
             raise ValueError(
                 f"position {batch.max_context - 1} is beyond the rotary table of {self.position.max_position}"
             )
+        if batch.adapters is not None:
+            return self._adapted(rows_complete(x), batch, view, writes, residual, next_norm, sums_parts)
         rows = x.shape[0]
         few = rows <= FUSED_ROWS or (rows <= FUSED_SMALL_ROWS and self.w_qkv.numel() <= FUSED_SMALL_WEIGHT)
         head_dim = self.kernel_head_dim  # what the kernels and the cache see
@@ -171,6 +185,19 @@ class Attention(Part):
                               view.block_table, view.k_pool, view.v_pool, self.num_heads, self.num_kv_heads,
                               head_dim, rotate=self.position.rotates, write_kv=writes, rotary_dim=rotary_dim)
         return self._attended(qkv, batch, view, residual, next_norm, sums_parts, unordered)
+
+    def _adapted(self, x: torch.Tensor, batch, view, writes: bool, residual: Optional[torch.Tensor], next_norm, sums_parts: bool):
+        """A step in which some rows have an adapter: the adapters' share joins q, k and v between the product and the rotation."""
+        rotary_dim = getattr(self.position, "rotary_dim", self.head_dim) if self.position.rotates else None
+        qkv = linear(x, self.w_qkv, self.b_qkv)
+        self.site_qkv.add(x, batch.adapters, qkv)
+        qkv = self.shape_projection(qkv, batch)
+        ops.rope_kv_write(qkv, self.cos, self.sin, batch.positions, batch.seq_of_token, batch.seq_slot, view.block_table, view.k_pool,
+                          view.v_pool, self.num_heads, self.num_kv_heads, self.kernel_head_dim, rotate=self.position.rotates,
+                          write_kv=writes, rotary_dim=rotary_dim)
+        context = attend(qkv, batch, view, self.num_heads, self.num_kv_heads, self.kernel_head_dim, self.window, self.scale)
+        return add_behind(self.site_o, context, batch.adapters, residual, lambda: linear(
+            context, self.w_o, self.b_o, into=residual, then_norm=next_norm, sums_parts=sums_parts and residual is not None))
 
     def _attended(self, qkv: torch.Tensor, batch, view, residual: Optional[torch.Tensor], next_norm, sums_parts: bool,
                   unordered: bool = False):

@@ -109,6 +109,9 @@ class Part:
     # ``adds_unordered``: ``forward`` takes ``unordered=``, and where that is true too (the layer's sums have no fixed order anyway)
     # its output may be added to the stream in parts that have none.  (Asked with ``declares``.)
     adds_unordered = False
+    # ``takes_adapters``: ``make_sites`` makes room for low-rank adapters beside the part's products, and ``forward`` adds them where
+    # the step has rows with one (``batch.adapters``; a feed-forward is handed ``adapters=``).  (Asked with ``declares``.)
+    takes_adapters = False
     # ``joins_products``: the part is one product in, something between, one product out.  Two such parts that read the
     # same rows and whose results are added may share both products: ``product_in()`` and ``product_out()`` give the
     # weights, and the part's own step between them takes the first product's rows and writes into a given matrix.

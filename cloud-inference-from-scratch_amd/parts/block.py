@@ -84,6 +84,7 @@ class PreNormBlock:
                 warm(rows)
 
     takes_added = True
+    takes_adapters = True  # what its parts do for rows that have one, it does
     unordered = False
 
     def forward(self, residual: torch.Tensor, pending: Optional[torch.Tensor], batch, view, writes: bool = True,
@@ -135,6 +136,8 @@ class PreNormBlock:
         extra = self._joins(self.feed_forward, residual if added or self.dtype != torch.float32 else None)
         if extra and declares(self.feed_forward, "sums_parts"):
             extra["sums_parts"] = True
+        if batch.adapters is not None:
+            extra["adapters"] = batch.adapters
         return residual, self.feed_forward.forward(x, **extra)
 
 

@@ -12,6 +12,7 @@ import torch
 
 from ..kernels import ops
 from ..weights.tensors import TensorSpec
+from .adapters import Module, Site, add_behind, rows_complete
 from .base import Part, register_part
 from .linear import linear
 
@@ -22,6 +23,7 @@ class GatedMLP(Part):
     takes_scaled_rows = True  # its first product applies the scale of rows that come without it
     takes_raw_rows = True  # its first product can make the norm of a few rows itself
     sums_parts = True  # its last product may come back as parts of K
+    takes_adapters = True  # rows of a step may each have a low-rank adapter beside its products
     gates_products = True  # its two products are the SiLU-gate one of ``w_gate_up`` and one of ``w_down``: a block may run them itself
     def __init__(self, hidden_size: int, intermediate_size: int, activation: str = "silu",
                  names: tuple[str, str, str] = ("gate_proj.weight", "up_proj.weight", "down_proj.weight")) -> None:
@@ -48,7 +50,23 @@ class GatedMLP(Part):
     def warm_up(self, rows: int) -> None:
         self.forward(torch.zeros((rows, self.hidden_size), dtype=self.w_down.dtype, device=self.w_down.device))
 
-    def forward(self, x, residual: Optional[torch.Tensor] = None, sums_parts: bool = False):
+    def make_sites(self, count: int, rank: int, scale: torch.Tensor) -> dict[str, Module]:
+        """Room for adapters beside the two products, by the names of the checkpoint's projections."""
+        inner, hidden = self.intermediate_size, self.hidden_size
+        self.site_gate_up = Site(hidden, (inner, inner), count, rank, self.dtype, self.device, scale)
+        self.site_down = Site(inner, (hidden,), count, rank, self.dtype, self.device, scale)
+        name = lambda index: self.names[index].removesuffix(".weight")  # noqa: E731
+        return {name(0): Module(self.site_gate_up, 0, hidden, inner), name(1): Module(self.site_gate_up, 1, hidden, inner),
+                name(2): Module(self.site_down, 0, inner, hidden)}
+
+    def forward(self, x, residual: Optional[torch.Tensor] = None, sums_parts: bool = False, adapters: Optional[torch.Tensor] = None):
+        if adapters is not None:
+            x = rows_complete(x)
+            gate_up = linear(x, self.w_gate_up)
+            self.site_gate_up.add(x, adapters, gate_up)
+            hidden = ops.silu_mul(gate_up)
+            return add_behind(self.site_down, hidden, adapters, residual, lambda: linear(
+                hidden, self.w_down, into=residual, sums_parts=sums_parts and residual is not None))
         return linear(linear(x, self.w_gate_up, epilogue="silu"), self.w_down, into=residual, sums_parts=sums_parts)
 
 

@@ -54,6 +54,7 @@ class DecoderModel:
         self.spec = spec
         self.blocks = _blocks(spec)
         self.final_norm = build_part("norm", spec.final_norm)
+        self.adapter_room: Any = None  # an AdapterRoom, where one was made
         self.embedding: torch.Tensor | None = None
         self.head: torch.Tensor | None = None
         # blocks that read what every earlier layer left (``keeps_history``) are handed a float32 tensor

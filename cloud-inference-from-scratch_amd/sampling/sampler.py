@@ -44,16 +44,20 @@ class Sampler:
             return uniform_for(request_seed, 0, index)
         return uniform_for(self.seed, serial, index)
 
-    def sample(self, logits: torch.Tensor, temperatures: Sequence[float],
-               uniforms: Sequence[float]) -> list[int]:
-        """One token per row of ``logits`` [n, vocab] (float32, on the GPU)."""
+    def sample(self, logits: torch.Tensor, temperatures: Sequence[float], uniforms: Sequence[float],
+               rules: Sequence[tuple[int, float, float] | None] | None = None) -> list[int]:
+        """One token per row of ``logits`` [n, vocab] (float32, on the GPU).  ``rules``: (top_k, top_p, min_p) of the rows that draw
+        under any."""
         if logits.shape[0] == 0:
             return []
-        return self.sample_on_device(logits, temperatures, uniforms).tolist()
+        return self.sample_on_device(logits, temperatures, uniforms, rules=rules).tolist()
 
     def sample_on_device(self, logits: torch.Tensor, temperatures: Sequence[float], uniforms: Sequence[float],
-                         out: torch.Tensor | None = None) -> torch.Tensor:
+                         out: torch.Tensor | None = None,
+                         rules: Sequence[tuple[int, float, float] | None] | None = None) -> torch.Tensor:
         """The same, left on the GPU (int32 [n], in ``out`` if given): nothing waits for the result."""
+        if rules is not None and any(rule is not None for rule in rules):
+            return self._sample_under_rules(logits, temperatures, uniforms, rules, out)
         if all(t == 0 for t in temperatures):
             return ops.sample(logits, out=out)
         # one page-locked block for both, copied without waiting: the decode steps that are started ahead of
@@ -63,3 +67,30 @@ class Sampler:
         staged = torch.tensor([*temperatures, *uniforms], dtype=torch.float32, pin_memory=pinned)
         on_device = staged.to(logits.device, non_blocking=True)
         return ops.sample(logits, on_device[:rows], on_device[rows:], out=out)
+
+    def _sample_under_rules(self, logits: torch.Tensor, temperatures: Sequence[float], uniforms: Sequence[float],
+                            rules: Sequence[tuple[int, float, float] | None], out: torch.Tensor | None) -> torch.Tensor:
+        """Some rows draw under rules.  The others keep the draw they have alone, whose sums are made in another way: a request's
+        tokens do not depend on what else is in the batch."""
+        rows = len(rules)
+        ruled = [rule is not None and t > 0 for rule, t in zip(rules, temperatures)]
+        given = [rule if on else (0, 1.0, 0.0) for rule, on in zip(rules, ruled)]
+        staged = torch.empty((6, rows), dtype=torch.float32, pin_memory=logits.device.type == "cuda")
+        staged[0] = torch.tensor([t if on else 0.0 for t, on in zip(temperatures, ruled)])
+        staged[1] = torch.tensor(uniforms)
+        staged[2] = torch.tensor([k for k, _p, _m in given], dtype=torch.int32).view(torch.float32)
+        staged[3] = torch.tensor([p for _k, p, _m in given])
+        staged[4] = torch.tensor([m for _k, _p, m in given])
+        staged[5] = torch.tensor([0.0 if on else t for t, on in zip(temperatures, ruled)])
+        row = staged.to(logits.device, non_blocking=True)
+        drawn = ops.sample(logits, row[0], row[1], top_k=row[2].view(torch.int32) if any(k for k, _p, _m in given) else None,
+                           top_p=row[3] if any(p < 1 for _k, p, _m in given) else None,
+                           min_p=row[4] if any(m > 0 for _k, _p, m in given) else None,
+                           out=out if all(ruled) else None)
+        if all(ruled):
+            return drawn
+        others = [t for t, on in zip(temperatures, ruled) if not on]
+        if any(t > 0 for t in others):
+            plain = ops.sample(logits, row[5], row[1])
+            drawn = torch.where(row[0] > 0, drawn, plain)  # (greedy rows are the same in both)
+        return drawn if out is None else out.copy_(drawn)
