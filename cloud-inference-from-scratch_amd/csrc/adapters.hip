@@ -103,6 +103,7 @@ struct Operand<float> {
 constexpr int kQuarters = 4;  // a wave's lanes hold 4 stretches of kLane k
 constexpr int kWaves = kThreads / kWave;
 constexpr int kTile = 16;
+constexpr int kGroup = 4;
 
 // The rows of a tile that have one adapter, first come first served: lane i learns the i-th of them.
 struct Gathered {
@@ -123,8 +124,9 @@ __device__ __forceinline__ Gathered gather(int id, u64 left) {
 
 // h_part[s, t, j]: the sums of part s of K.  grid: (parts, row tiles, column groups x slots).  A workgroup takes every
 // `slots`-th of its tile's adapters.  K falls into chunks whose length depends on K alone; four waves share a chunk's k and join
-// their sums through LDS, chunks are added one after the other.  A part is one chunk (few rows: as many workgroups as there
-// are) or all of them (many rows: one part): either way h is the same sum in the same order, whatever rows are beside it.
+// their sums through LDS, chunks are added one after the other in groups of kGroup, and the groups one after the other.  A part is
+// one chunk (few rows: as many workgroups as there are) or a group of them (many rows: fewer sums to write and read): either
+// way h is the same sum in the same order, whatever rows are beside it.
 template <typename T, int C, int R>
 __device__ __forceinline__ void down_rows(const Gathered& g, const T* __restrict__ x, long ldx, const T* __restrict__ down,
                                           float* __restrict__ part, int row0, int inner, int j0, int k, int k_begin, int k_end,
@@ -226,7 +228,7 @@ __device__ __forceinline__ void down_rows(const Gathered& g, const T* __restrict
         }
 }
 
-template <typename T, int C>
+template <typename T, int C, bool kOneTile>  // kOneTile: tile_rows is 16 (a third of the registers: the form for many rows)
 __global__ void __launch_bounds__(kThreads)
 adapter_down_tiles(const T* __restrict__ x, long ldx, const T* __restrict__ down, const int* __restrict__ adapter,
                    float* __restrict__ h_part, int rows, int inner, int k, int adapters, int tile_rows, int slots, int chunk,
@@ -243,12 +245,14 @@ adapter_down_tiles(const T* __restrict__ x, long ldx, const T* __restrict__ down
         const Gathered g = gather(id, left);
         left &= ~__ballot(id == g.adapter);
         if (number % slots != slot) continue;
-        if (g.count <= kTile)
+        if (kOneTile || g.count <= kTile)
             down_rows<T, C, 1>(g, x, ldx, down, part, row0, inner, j0, k, k_begin, k_end, chunk, s_sum);
-        else if (g.count <= 2 * kTile)
-            down_rows<T, C, 2>(g, x, ldx, down, part, row0, inner, j0, k, k_begin, k_end, chunk, s_sum);
-        else
-            down_rows<T, C, 4>(g, x, ldx, down, part, row0, inner, j0, k, k_begin, k_end, chunk, s_sum);
+        else if constexpr (!kOneTile) {
+            if (g.count <= 2 * kTile)
+                down_rows<T, C, 2>(g, x, ldx, down, part, row0, inner, j0, k, k_begin, k_end, chunk, s_sum);
+            else
+                down_rows<T, C, 4>(g, x, ldx, down, part, row0, inner, j0, k, k_begin, k_end, chunk, s_sum);
+        }
     }
 }
 
@@ -394,6 +398,25 @@ struct Share {
     }
 };
 
+// Four numbers of h: the parts, `apart` floats from each other, in the one order (chunks: by groups).
+__device__ __forceinline__ quad_t sum_of_parts(const float* at, size_t apart, int parts, bool chunks) {
+    quad_t sum = {0.f, 0.f, 0.f, 0.f};
+    if (!chunks) {
+#pragma unroll 4
+        for (int s = 0; s < parts; ++s) sum += *reinterpret_cast<const quad_t*>(at + s * apart);
+        return sum;
+    }
+#pragma unroll 2
+    for (int s = 0; s < parts; s += kGroup) {
+        quad_t part[kGroup] = {};
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i)
+            if (s + i < parts) part[i] = *reinterpret_cast<const quad_t*>(at + (s + i) * apart);
+        sum += ((part[0] + part[1]) + part[2]) + part[3];
+    }
+    return sum;
+}
+
 // Who of a row tile has which adapter.
 struct Order {
     int id[kWave], order[kWave];  // the rows' adapters (-1: none, or not this workgroup's); the rows by adapter,
@@ -438,19 +461,16 @@ struct Rows {
     static constexpr int kLd = kWidth + 16 / sizeof(store_t);  // (rows a little apart, so that 16 of them do not share their banks)
     store_t number[kHalves][kWave][kLd];
 
-    __device__ __forceinline__ void add_parts(const Order& tile, const float* h_part, int parts, const float* scale, int row0, int rows,
-                                              int inner, int from, int rank) {
+    __device__ __forceinline__ void add_parts(const Order& tile, const float* h_part, int parts, bool chunks, const float* scale, int row0,
+                                              int rows, int inner, int from, int rank) {
         constexpr int kFours = kWidth / 4;
         for (int item = threadIdx.x; item < kWave * kFours; item += kThreads) {
             const int row = item / kFours, r = item % kFours * 4, a = tile.id[row];
             if (a < 0) continue;
             quad_t sum = {0.f, 0.f, 0.f, 0.f};
-            if (r < rank) {
-                const float* at = h_part + static_cast<size_t>(row0 + row) * inner + from + r;
-#pragma unroll 8
-                for (int s = 0; s < parts; ++s) sum += *reinterpret_cast<const quad_t*>(at + static_cast<size_t>(s) * rows * inner);
-                sum *= scale[a];
-            }
+            if (r < rank)
+                sum = sum_of_parts(h_part + static_cast<size_t>(row0 + row) * inner + from + r, static_cast<size_t>(rows) * inner, parts, chunks) *
+                      scale[a];
 #pragma unroll
             for (int e = 0; e < 4; ++e) Inner<T>::put(&number[0][row][r + e], kWave * kLd, sum[e]);
         }
@@ -478,7 +498,7 @@ struct Columns {
 // are added.
 template <typename T, typename S, int kSteps>
 __global__ void __launch_bounds__(kThreads)
-adapter_up_rows(const float* __restrict__ h_part, int parts, const T* __restrict__ up, const float* __restrict__ scale,
+adapter_up_rows(const float* __restrict__ h_part, int parts, bool chunks, const T* __restrict__ up, const float* __restrict__ scale,
                 const int* __restrict__ adapter, const S* into, long ld_into, S* out, long ld_out, int rows, int inner, int n, int rank,
                 int adapters, Pieces pieces, int block, int slots, bool wide) {
     __shared__ Order tile;
@@ -499,7 +519,7 @@ adapter_up_rows(const float* __restrict__ h_part, int parts, const T* __restrict
     };
     int number = wave;
     if (number < shares) ask(number);
-    h.add_parts(tile, h_part, parts, scale, row0, rows, inner, columns.piece * rank, rank);
+    h.add_parts(tile, h_part, parts, chunks, scale, row0, rows, inner, columns.piece * rank, rank);
     while (number < shares) {
         share.finish(h.number, columns.end, into, ld_into, out, ld_out);
         number += kWaves;
@@ -512,7 +532,7 @@ adapter_up_rows(const float* __restrict__ h_part, int parts, const T* __restrict
 // registers.  The strip's weights pass through LDS, which all four read, a strip ahead of its use.
 template <typename T, typename S, int kSteps>
 __global__ void __launch_bounds__(kThreads, 4)
-adapter_up_strips(const float* __restrict__ h_part, int parts, const T* __restrict__ up, const float* __restrict__ scale,
+adapter_up_strips(const float* __restrict__ h_part, int parts, bool chunks, const T* __restrict__ up, const float* __restrict__ scale,
                   const int* __restrict__ adapter, const S* into, long ld_into, S* out, long ld_out, int rows, int inner, int n, int rank,
                   int adapters, Pieces pieces, int block, bool wide) {
     typedef Operand<T> Op;
@@ -581,10 +601,7 @@ adapter_up_strips(const float* __restrict__ h_part, int parts, const T* __restri
 #pragma unroll
             for (int e = 0; e < Op::kLane; e += 4) {
                 quad_t sum = {0.f, 0.f, 0.f, 0.f};
-                if (r + e < rank) {
-                    for (int p = 0; p < parts; ++p) sum += *reinterpret_cast<const quad_t*>(at + e + static_cast<size_t>(p) * rows * inner);
-                    sum *= factor;
-                }
+                if (r + e < rank) sum = sum_of_parts(at + e, static_cast<size_t>(rows) * inner, parts, chunks) * factor;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) Inner<T>::put(&both[0][e + i], Op::kLane, sum[i]);
             }
@@ -597,7 +614,7 @@ adapter_up_strips(const float* __restrict__ h_part, int parts, const T* __restri
     ask_weights(0);
     ask_rows(0);
     if (many)
-        s_h.add_parts(tile, h_part, parts, scale, row0, rows, inner, columns.piece * rank, rank);
+        s_h.add_parts(tile, h_part, parts, chunks, scale, row0, rows, inner, columns.piece * rank, rank);
     else
         ask_h();
     for (int number = 0; number < total; ++number) {
@@ -653,16 +670,21 @@ adapter_up_strips(const float* __restrict__ h_part, int parts, const T* __restri
 
 struct Plan {
     int chunk, parts, tile_rows, slots, block, up_slots;
+    bool chunks(int k) const { return parts == (k + chunk - 1) / chunk; }
 };
 
 template <typename T, int C>
 int launch_down(hipStream_t s, const T* x, long ldx, const T* down, const int* adapter, float* h, int rows, int k, int inner, int adapters,
                 const Plan& plan) {
-    const int part_k = plan.parts == 1 ? (k + plan.chunk - 1) / plan.chunk * plan.chunk : plan.chunk;
+    const int part_k = plan.chunks(k) ? plan.chunk : kGroup * plan.chunk;
     const int groups = (inner + C * kTile - 1) / (C * kTile);
     const dim3 grid(plan.parts, (rows + plan.tile_rows - 1) / plan.tile_rows, groups * plan.slots);
-    adapter_down_tiles<T, C><<<grid, kThreads, 0, s>>>(x, ldx, down, adapter, h, rows, inner, k, adapters, plan.tile_rows, plan.slots,
-                                                       plan.chunk, part_k);
+    if (plan.tile_rows == kTile)
+        adapter_down_tiles<T, C, true><<<grid, kThreads, 0, s>>>(x, ldx, down, adapter, h, rows, inner, k, adapters, plan.tile_rows,
+                                                                plan.slots, plan.chunk, part_k);
+    else
+        adapter_down_tiles<T, C, false><<<grid, kThreads, 0, s>>>(x, ldx, down, adapter, h, rows, inner, k, adapters, plan.tile_rows,
+                                                                 plan.slots, plan.chunk, part_k);
     return cie_after_launch();
 }
 
@@ -690,7 +712,7 @@ int run_tiles(hipStream_t s, const void* x_, long ldx, const void* down_, const 
     if (plan.up_slots > 0) {
 #define CIE_UP(STEPS)                                                                                                              \
     adapter_up_rows<T, S, STEPS><<<dim3(row_tiles, blocks, plan.up_slots), kThreads, 0, s>>>(                                          \
-        h, plan.parts, up, scale, adapter, into, ld_into, out, ld_out, rows, inner, n, rank, adapters, pieces, plan.block, plan.up_slots, wide)
+        h, plan.parts, plan.chunks(k), up, scale, adapter, into, ld_into, out, ld_out, rows, inner, n, rank, adapters, pieces, plan.block, plan.up_slots, wide)
         if (rank <= kStep)
             CIE_UP(1);
         else if (rank <= 2 * kStep)
@@ -702,7 +724,7 @@ int run_tiles(hipStream_t s, const void* x_, long ldx, const void* down_, const 
 #undef CIE_UP
     } else {
 #define CIE_UP(STEPS)                                                                                                        \
-    adapter_up_strips<T, S, STEPS><<<dim3(row_tiles, blocks), kThreads, 0, s>>>(h, plan.parts, up, scale, adapter, into, ld_into, out, \
+    adapter_up_strips<T, S, STEPS><<<dim3(row_tiles, blocks), kThreads, 0, s>>>(h, plan.parts, plan.chunks(k), up, scale, adapter, into, ld_into, out, \
                                                                               ld_out, rows, inner, n, rank, adapters, pieces, plan.block, wide)
         if (rank <= kStep)
             CIE_UP(1);
@@ -720,7 +742,7 @@ int run_tiles(hipStream_t s, const void* x_, long ldx, const void* down_, const 
 // dtype: of x, down and up; out_dtype: of into and out (dtype, or float32).  c1, c2, c3: where the second and later pieces begin
 // (n where there is none).  out may be into.  parts = 0: the kernels that take any shape (h: rows * pieces * rank floats).  Else the
 // tiles, which take a rank that is a multiple of 4 and rows of x and down in 16-byte pieces: K in chunks of `chunk`, each of them
-// a part or all of them one (h: as many floats for each part), `down` in tiles of tile_rows (16 to 64) rows and `slots` workgroups
+// a part or each four (h: as many floats for each part), `down` in tiles of tile_rows (16 to 64) rows and `slots` workgroups
 // for a tile's adapters, `up` in blocks of `block` columns; up_slots > 0: in the form for few
 // rows, with so many workgroups for the adapters of a tile of 64 rows, 0: in the form for many (a rank of up to 64).
 CIE_API int cie_lora_add(void* stream, int dtype, int out_dtype, const void* x, long ldx, const void* down, const void* up,
@@ -742,7 +764,7 @@ CIE_API int cie_lora_add(void* stream, int dtype, int out_dtype, const void* x, 
                            reinterpret_cast<uintptr_t>(down) % 16 == 0 && reinterpret_cast<uintptr_t>(up) % 16 == 0 &&
                            reinterpret_cast<uintptr_t>(h) % 16 == 0;
         const int share = 256 / size;  // (the k that a workgroup's four waves take at a time)
-        if (!lines || rank % 4 || chunk < 2 * share || chunk % (2 * share) || (parts != 1 && parts != (k + chunk - 1) / chunk) || tile_rows < 16 ||
+        if (!lines || rank % 4 || chunk < 2 * share || chunk % (2 * share) || (parts != (k + chunk - 1) / chunk && parts != (k + kGroup * chunk - 1) / (kGroup * chunk)) || tile_rows < 16 ||
             tile_rows > kWave || tile_rows % kTile || slots < 1 || slots > kWave || block < kWave || block % kWave || up_slots < 0 ||
             up_slots > kWave || (up_slots == 0 && rank > 64))
             return CIE_BAD_ARGUMENT;

@@ -1481,9 +1481,9 @@ def sample(logits: torch.Tensor, temperature: Optional[torch.Tensor] = None,
 
 def _on_current_gpu(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
     """All operands on the GPU whose stream the kernel will run on."""
-    index = first.get_device()
-    if index != torch._C._cuda_getDevice():
-        raise ValueError(f"the operands live on {first.device}, and cuda:{torch._C._cuda_getDevice()} is the current device")
+    index = torch._C._cuda_getDevice()
+    if first.get_device() != index:
+        raise ValueError(f"the operands live on {first.device}, and cuda:{index} is the current device")
     for other in others:
         if other is not None and other.get_device() != index:
             raise ValueError(f"operands on {first.device} and {other.device}")
@@ -1499,9 +1499,10 @@ def _logit_rows(logits: torch.Tensor) -> tuple[int, int]:
 
 
 def _per_row(name: str, t: torch.Tensor, dtype: torch.dtype, rows: int) -> None:
+    if t.dtype is dtype and t.is_cuda and t.dim() == 1 and t.shape[0] == rows and t.is_contiguous():
+        return  # (one test for what nearly all calls bring: these operators are called several times a layer)
     _gpu(name, t, dtype, 1)
-    if t.shape[0] != rows:
-        raise ValueError(f"{name} must be [{rows}], is {list(t.shape)}")
+    raise ValueError(f"{name} must be [{rows}], is {list(t.shape)}")
 
 
 MAX_RULE_ROWS, MAX_RULE_VOCAB = 65535, 1 << 23
@@ -1518,22 +1519,26 @@ def _sample_rules(logits, temperature, uniform, out, top_k, top_p, min_p) -> tor
         raise ValueError(f"up to {MAX_RULE_ROWS} rows of {MAX_RULE_VOCAB} logits, not {rows} of {vocab}")
     _per_row("temperature", temperature, torch.float32, rows)
     _per_row("uniform", uniform, torch.float32, rows)
-    for name, rule, dtype in (("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
-        if rule is not None:
-            _per_row(name, rule, dtype, rows)
+    words = RULES_PART_WORDS * -(-vocab // RULES_PART)
+    if top_k is not None:
+        _per_row("top_k", top_k, torch.int32, rows)
+    if top_p is not None:
+        _per_row("top_p", top_p, torch.float32, rows)
+    if min_p is not None:
+        _per_row("min_p", min_p, torch.float32, rows)
+    if top_p is not None or min_p is not None:
+        words += RULES_ROW_WORDS
     if out is None:
         out = torch.empty((rows,), dtype=torch.int32, device=logits.device)
-    _per_row("out", out, torch.int32, rows)
+    else:
+        _per_row("out", out, torch.int32, rows)
     _on_current_gpu(logits, temperature, uniform, top_k, top_p, min_p, out)
     if rows == 0:
         return out
-    words = RULES_PART_WORDS * -(-vocab // RULES_PART)
-    if top_p is not None or min_p is not None:
-        words += RULES_ROW_WORDS
-    work = torch.empty(rows * words, dtype=torch.int64, device=logits.device)
+    work = torch.empty((rows * words,), dtype=torch.int64, device=logits.device)
     _run("cie_sample_rules", load_library().cie_sample_rules(
-        _stream(), _ptr(logits), _ptr(temperature), _ptr(uniform), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(out), _ptr(work),
-        _i(rows), _i(vocab), _i(_ld(logits)), _i(max(1, RULES_SPREAD // rows))))
+        _stream(), logits.data_ptr(), temperature.data_ptr(), uniform.data_ptr(), _ptr(top_k), _ptr(top_p), _ptr(min_p), out.data_ptr(),
+        work.data_ptr(), rows, vocab, _ld(logits), max(1, RULES_SPREAD // rows)))
     return out
 
 
@@ -1551,7 +1556,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, out: Optional[tor
         raise ValueError(f"up to {MAX_RULE_ROWS} rows of {1 << 30} logits, not {rows} of {vocab}")
     if out is None:
         out = torch.empty((rows,), dtype=torch.float32, device=logits.device)
-    _per_row("out", out, torch.float32, rows)
+    else:
+        _per_row("out", out, torch.float32, rows)
     _on_current_gpu(logits, tokens, out)
     if rows == 0:
         return out
@@ -1574,13 +1580,14 @@ def plan_lora(rows: int, k: int, n: int, inner: int, rank: int, count: int, shar
     second product, workgroups for the adapters of its 64 rows) of :func:`lora_add`.  ``share``: the k that a workgroup takes at
     a time.  The chunk goes by K alone, so that the sums do."""
     chunk = max(1, -(-k // (32 * share))) * 2 * share
-    few = rows * inner * -(-k // chunk) <= 1 << 20
+    chunks = -(-k // chunk)
+    parts = chunks if rows * inner * chunks <= 1 << 20 else -(-chunks // 4)
     tile_rows = 64 if rows <= 128 else 16
     slots = min(count, rows, 16 if rows <= 128 else 2)
-    parts = -(-k // chunk) if few else 1
     tiles, strips = -(-rows // 64), -(-n // 128)
-    up_slots = 0 if rows > 128 and rank <= 64 else min(count, rows, 8)
-    block = 128 * max(1, -(-strips * tiles // (4 * units)))
+    many = tiles * strips >= 4 * units and rank <= 64
+    up_slots = 0 if many else min(count, rows, 4)
+    block = 128 * (-(-strips * tiles // (4 * units)) if many else 1)
     return chunk, parts, tile_rows, slots, block, up_slots
 
 
@@ -1598,17 +1605,18 @@ def lora_add(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale: torch
         raise ValueError(f"x {tuple(x.shape)} and into {tuple(into.shape)} must be matrices")
     rows, k = x.shape
     n = into.shape[1]
-    code = _code(x.dtype)
-    _row_view("x", x, (rows, k), (x.dtype,))
-    _row_view("into", into, (rows, n), (x.dtype, torch.float32))
+    dtype, out_dtype = x.dtype, into.dtype
+    code = _code(dtype)
+    _row_view("x", x, (rows, k), (dtype,))
+    _row_view("into", into, (rows, n), (dtype, torch.float32))
     columns = (n,) if columns is None else tuple(columns)
     pieces = len(columns)
     if not 1 <= pieces <= MAX_ADAPTER_PIECES or min(columns) < 1 or sum(columns) != n:
         raise ValueError(f"columns {columns} must be 1 to {MAX_ADAPTER_PIECES} positive widths that add up to {n}")
-    _gpu("down", down, x.dtype, 3)
-    _gpu("up", up, x.dtype, 3)
+    _gpu("down", down, dtype, 3)
+    _gpu("up", up, dtype, 3)
     count, n_up, rank = up.shape
-    if not (1 <= rank <= MAX_ADAPTER_RANK and n_up == n and tuple(down.shape) == (count, pieces * rank, k) and count >= 1 and k >= 1):
+    if not (1 <= rank <= MAX_ADAPTER_RANK and n_up == n and down.shape == (count, pieces * rank, k) and count >= 1 and k >= 1):
         raise ValueError(f"down {tuple(down.shape)} and up {tuple(up.shape)} do not fit rows of {k}, {n} columns in {pieces} pieces "
                          f"and a rank of 1 to {MAX_ADAPTER_RANK}")
     _per_row("scale", scale, torch.float32, count)
@@ -1616,24 +1624,24 @@ def lora_add(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale: torch
     if out is None:
         out = into
     else:
-        _row_view("out", out, (rows, n), (into.dtype,))
+        _row_view("out", out, (rows, n), (out_dtype,))
     _on_current_gpu(x, down, up, scale, adapters, into, out)
     if rows > 65535:
         raise ValueError(f"up to 65,535 rows, not {rows}")
     if rows == 0:
         return out
-    size = x.element_size()
-    if (rank % 4 == 0 and k * size % 16 == 0 and _ld(x) * size % 16 == 0 and x.data_ptr() % 16 == 0 and down.data_ptr() % 16 == 0
-            and up.data_ptr() % 16 == 0):
+    size = 4 if code == F32 else 2
+    ldx, x_at, down_at, up_at = _ld(x), x.data_ptr(), down.data_ptr(), up.data_ptr()
+    if rank % 4 == 0 and (k * size | ldx * size | x_at | down_at | up_at) % 16 == 0:
         plan = plan_lora(rows, k, n, pieces * rank, rank, count, 256 // size, compute_units())
     else:  # (a rank or a row that 16-byte loads do not take)
         plan = (0, 0, 0, 0, 0, 0)
-    inner = torch.empty(max(1, plan[1]) * rows * pieces * rank, dtype=torch.float32, device=x.device)
-    begins = [sum(columns[:p]) for p in range(1, pieces)] + [n] * (MAX_ADAPTER_PIECES - pieces)
+    inner = torch.empty((max(1, plan[1]) * rows * pieces * rank,), dtype=torch.float32, device=x.device)
+    c1 = columns[0]
+    c2 = c1 + columns[1] if pieces > 1 else n
     _run("cie_lora_add", load_library().cie_lora_add(
-        _stream(), _i(code), _i(_code(into.dtype)), _ptr(x), _i(_ld(x)), _ptr(down), _ptr(up), _ptr(scale), _ptr(adapters),
-        _ptr(into), _i(_ld(into)), _ptr(out), _i(_ld(out)), _ptr(inner), _i(rows), _i(k), _i(n), _i(rank), _i(count), _i(pieces),
-        _i(begins[0]), _i(begins[1]), _i(begins[2]), *plan))
+        _stream(), code, _CODES[out_dtype], x_at, ldx, down_at, up_at, scale.data_ptr(), adapters.data_ptr(), into.data_ptr(), _ld(into),
+        out.data_ptr(), _ld(out), inner.data_ptr(), rows, k, n, rank, count, pieces, c1, c2, c2 + columns[2] if pieces > 2 else n, *plan))
     return out
 
 
