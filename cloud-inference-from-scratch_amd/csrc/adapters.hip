@@ -104,6 +104,7 @@ constexpr int kQuarters = 4;  // a wave's lanes hold 4 stretches of kLane k
 constexpr int kWaves = kThreads / kWave;
 constexpr int kTile = 16;
 constexpr int kGroup = 4;
+constexpr int kXcds = 8;
 
 // The rows of a tile that have one adapter, first come first served: lane i learns the i-th of them.
 struct Gathered {
@@ -527,14 +528,20 @@ adapter_up_rows(const float* __restrict__ h_part, int parts, bool chunks, const 
     }
 }
 
-// Many rows.  grid: (row tiles, column blocks of the pieces).  A workgroup goes through its strips of columns, and in each through
+// Many rows.  grid: row tiles x column blocks of the pieces, rounded up to whole turns of the XCDs: each XCD has a run of them in
+// which the row tiles of a column block follow each other, so that its L2 holds the block's weights (dealt out one by one, every
+// XCD fetched all weights: 103 us for 2,048 rows of 37,888 columns at rank 64).  A workgroup goes through its strips of columns, and in each through
 // its tile's adapters (of a prompt there is one); each of its four waves has 16 of the adapter's rows, whose h it keeps in
 // registers.  The strip's weights pass through LDS, which all four read, a strip ahead of its use.
-template <typename T, typename S, int kSteps>
+//
+// The loop over whole strips has no branch around a load or store: rows that are not there have an offset behind their buffer's end,
+// which drops them.  The wait for a strip's weights then leaves the rows and stores behind them under way; with branches the
+// compiler has to wait for all of them, once a strip.
+template <typename T, typename S, int kSteps, bool kEven>  // kEven: the rank is a multiple of a lane's numbers
 __global__ void __launch_bounds__(kThreads, 4)
 adapter_up_strips(const float* __restrict__ h_part, int parts, bool chunks, const T* __restrict__ up, const float* __restrict__ scale,
                   const int* __restrict__ adapter, const S* into, long ld_into, S* out, long ld_out, int rows, int inner, int n, int rank,
-                  int adapters, Pieces pieces, int block, bool wide) {
+                  int adapters, Pieces pieces, int block, int row_tiles, int blocks, bool wide) {
     typedef Operand<T> Op;
     typedef typename Inner<T>::store_t store_t;
     constexpr int kOwn = Piece<S>::kNumbers, kStrip = kTile * kOwn, kLoads = kSteps * kQuarters, kMine = kStrip * kLoads / kThreads;
@@ -551,44 +558,62 @@ adapter_up_strips(const float* __restrict__ h_part, int parts, bool chunks, cons
     __shared__ __align__(16) char lds[sizeof(Weights) + kSecond];
     Weights* const s_w = reinterpret_cast<Weights*>(lds);
     RowsT& s_h = *reinterpret_cast<RowsT*>(lds + sizeof(Weights));
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, quarter = lane / kTile, row0 = blockIdx.x * kWave;
-    const Columns columns(pieces, blockIdx.y, block);
+    const int number_of_all = blockIdx.x % kXcds * (gridDim.x / kXcds) + blockIdx.x / kXcds;
+    if (number_of_all >= row_tiles * blocks) return;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, quarter = lane / kTile, row0 = number_of_all % row_tiles * kWave;
+    const Columns columns(pieces, number_of_all / row_tiles, block);
     tile.sort_rows(adapter, row0, rows, adapters, 1, 0, static_cast<const void*>(into) != static_cast<const void*>(out));
     if (tile.count == 0) return;
     into += static_cast<size_t>(row0) * ld_into;
     out += static_cast<size_t>(row0) * ld_out;
+    // (wide: the last row of a tile ends below 2 GB)
+    const unsigned last = min(kWave, rows - row0) - 1;
+    constexpr int kNowhere = static_cast<int>(0x80000000u);
+    const __amdgpu_buffer_rsrc_t of_into = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<S*>(into), 0, wide ? (last * static_cast<unsigned>(ld_into) + n) * static_cast<unsigned>(sizeof(S)) : 0, 0x00027000);
+    const __amdgpu_buffer_rsrc_t of_out = __builtin_amdgcn_make_buffer_rsrc(
+        out, 0, wide ? (last * static_cast<unsigned>(ld_out) + n) * static_cast<unsigned>(sizeof(S)) : 0, 0x00027000);
     const int groups = tile.count, total = (columns.end - columns.begin + kStrip - 1) / kStrip * groups;
+    const int whole = wide ? (columns.end - columns.begin) / kStrip * groups : 0;
+    const bool many = groups > 1;
 
     typename Op::type staged[kMine], h[kHalves][kSteps];
     words_t old[4];
     const auto ask_weights = [&](int number) {
-        const int a = tile.id[tile.order[tile.group[number % groups]]];
-        if (a < 0) return;
+        const int a = max(0, tile.id[tile.order[tile.group[number % groups]]]);  // (rows without an adapter: not used)
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
             const int item = i * kThreads + threadIdx.x, c = min(columns.begin + number / groups * kStrip + item / kLoads, columns.end - 1);
-            staged[i] = up_numbers(up + (static_cast<size_t>(a) * n + c) * rank, item % kLoads * Op::kLane, rank);
+            const int from = item % kLoads * Op::kLane;
+            const T* row = up + (static_cast<size_t>(a) * n + c) * rank;
+            if constexpr (kEven) {
+                staged[i] = *reinterpret_cast<const typename Op::type*>(row + (from < rank ? from : 0));
+                if (from >= rank) staged[i] = typename Op::type{};
+            } else {
+                staged[i] = up_numbers(row, from, rank);
+            }
         }
     };
     // (column c lies where the lane that computes it reads without sharing banks)
-    const auto put_weights = [&](int number) {  // (of the buffer)
+    const auto put_weights = [&](int buffer) {
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
             const int item = i * kThreads + threadIdx.x, c = item / kLoads;
-            *reinterpret_cast<typename Op::type*>(&s_w[number].number[c % kOwn * kTile + c / kOwn][item % kLoads * Op::kLane]) = staged[i];
+            *reinterpret_cast<typename Op::type*>(&s_w[buffer].number[c % kOwn * kTile + c / kOwn][item % kLoads * Op::kLane]) = staged[i];
         }
+    };
+    const auto offset = [&](int number, int i, long ld) {
+        const int from = tile.group[number % groups], which = wave * kTile + quarter * 4 + i;
+        const int first = columns.begin + number / groups * kStrip + lane % kTile * kOwn;
+        return which < tile.group[number % groups + 1] - from
+                   ? (tile.order[from + which] * static_cast<int>(ld) + first) * static_cast<int>(sizeof(S))
+                   : kNowhere;
     };
     const auto ask_rows = [&](int number) {
-        const int from = tile.group[number % groups], count = tile.group[number % groups + 1] - from;
-        const int first = columns.begin + number / groups * kStrip + lane % kTile * kOwn;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int which = wave * kTile + quarter * 4 + i;
-            if (wide && first + kOwn <= columns.end && which < count)
-                old[i] = *reinterpret_cast<const words_t*>(into + static_cast<size_t>(tile.order[from + which]) * ld_into + first);
-        }
+        for (int i = 0; i < 4; ++i)
+            old[i] = __builtin_bit_cast(words_t, __builtin_amdgcn_raw_buffer_load_b128(of_into, offset(number, i, ld_into), 0, 0));
     };
-    const bool many = groups > 1;
     const auto ask_h = [&]() {  // of a tile's one adapter
         const int row = tile.order[min(wave * kTile + lane % kTile, tile.group[1] - 1)], a = tile.id[row];
         if (a < 0) return;
@@ -611,60 +636,77 @@ adapter_up_strips(const float* __restrict__ h_part, int parts, bool chunks, cons
                 for (int e = 0; e < Op::kLane; ++e) h[half][s][e] = both[half][e];
         }
     };
+    // the strip's weights are in LDS, the next ones are asked for: what the wave's 16 rows gain
+    const auto gains = [&](int number, quad_t(&acc)[kOwn]) {
+        const int buffer = many ? 0 : number & 1;
+        if (many) __syncthreads();  // (the buffer has been read by all)
+        put_weights(buffer);
+        __syncthreads();  // (and the other buffer has been read by all)
+        ask_weights(min(number + 1, total - 1));
+        const int from = tile.group[number % groups], count = tile.group[number % groups + 1] - from;
+        if (wave * kTile >= count) return;
+        if (many) {
+            const int row = tile.order[from + min(wave * kTile + lane % kTile, count - 1)];
+#pragma unroll
+            for (int half = 0; half < kHalves; ++half)
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s)
+                    h[half][s] = *reinterpret_cast<const typename Op::type*>(&s_h.number[half][row][(s * kQuarters + quarter) * Op::kLane]);
+        }
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j) {
+                const typename Op::type weights =
+                    *reinterpret_cast<const typename Op::type*>(&s_w[buffer].number[j * kTile + lane % kTile][(s * kQuarters + quarter) * Op::kLane]);
+#pragma unroll
+                for (int half = 0; half < kHalves; ++half) acc[j] = Op::mac(h[half][s], weights, acc[j]);
+            }
+    };
     ask_weights(0);
     ask_rows(0);
     if (many)
         s_h.add_parts(tile, h_part, parts, chunks, scale, row0, rows, inner, columns.piece * rank, rank);
     else
         ask_h();
-    for (int number = 0; number < total; ++number) {
-        if (many) __syncthreads();  // (the buffer has been read by all)
-        const int buffer = many ? 0 : number & 1;
-        put_weights(buffer);
-        __syncthreads();  // (and the other buffer has been read by all)
-        if (number + 1 < total) ask_weights(number + 1);
+    int number = 0;
+    for (; number < whole; ++number) {
+        quad_t acc[kOwn] = {};
+        gains(number, acc);
+        const bool has = tile.id[tile.order[tile.group[number % groups]]] >= 0;
+        words_t now[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float more[kOwn];
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j) more[j] = acc[j][i];
+            const words_t sum = Piece<S>::sum(old[i], more);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) now[i][w] = has ? sum[w] : old[i][w];
+        }
+        ask_rows(min(number + 1, total - 1));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(int __attribute__((ext_vector_type(4))), now[i]), of_out,
+                                                   offset(number, i, ld_out), 0, 0);
+    }
+    // the columns behind the last whole strip, or rows that 16-byte pieces do not take
+    for (; number < total; ++number) {
+        quad_t acc[kOwn] = {};
+        gains(number, acc);
         const int from = tile.group[number % groups], count = tile.group[number % groups + 1] - from, a = tile.id[tile.order[from]];
         const int first = columns.begin + number / groups * kStrip + lane % kTile * kOwn;
-        const bool whole = wide && first + kOwn <= columns.end;
-        quad_t acc[kOwn] = {};
-        if (a >= 0 && wave * kTile < count) {
-            if (many) {
-                const int row = tile.order[from + min(wave * kTile + lane % kTile, count - 1)];
-#pragma unroll
-                for (int half = 0; half < kHalves; ++half)
-#pragma unroll
-                    for (int s = 0; s < kSteps; ++s)
-                        h[half][s] = *reinterpret_cast<const typename Op::type*>(&s_h.number[half][row][(s * kQuarters + quarter) * Op::kLane]);
-            }
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-                for (int j = 0; j < kOwn; ++j) {
-                    const typename Op::type weights =
-                        *reinterpret_cast<const typename Op::type*>(&s_w[buffer].number[j * kTile + lane % kTile][(s * kQuarters + quarter) * Op::kLane]);
-#pragma unroll
-                    for (int half = 0; half < kHalves; ++half) acc[j] = Op::mac(h[half][s], weights, acc[j]);
-                }
-        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int which = wave * kTile + quarter * 4 + i;
             if (which >= count) continue;
             const int row = tile.order[from + which];
-            S* to = out + static_cast<size_t>(row) * ld_out + first;
-            if (whole) {
-                float more[kOwn];
-#pragma unroll
-                for (int j = 0; j < kOwn; ++j) more[j] = acc[j][i];
-                *reinterpret_cast<words_t*>(to) = a >= 0 ? Piece<S>::sum(old[i], more) : old[i];
-                continue;
-            }
             const S* source = into + static_cast<size_t>(row) * ld_into + first;
+            S* to = out + static_cast<size_t>(row) * ld_out + first;
 #pragma unroll
             for (int j = 0; j < kOwn; ++j)
                 if (first + j < columns.end) to[j] = a >= 0 ? from_float<S>(to_float(source[j]) + acc[j][i]) : source[j];
         }
-        if (number + 1 < total) ask_rows(number + 1);
     }
 }
 
@@ -723,16 +765,26 @@ int run_tiles(hipStream_t s, const void* x_, long ldx, const void* down_, const 
             CIE_UP(8);
 #undef CIE_UP
     } else {
-#define CIE_UP(STEPS)                                                                                                        \
-    adapter_up_strips<T, S, STEPS><<<dim3(row_tiles, blocks), kThreads, 0, s>>>(h, plan.parts, plan.chunks(k), up, scale, adapter, into, ld_into, out, \
-                                                                              ld_out, rows, inner, n, rank, adapters, pieces, plan.block, wide)
-        if (rank <= kStep)
+        const bool near = (static_cast<double>(kWave) * (ld_into > ld_out ? ld_into : ld_out) + n) * sizeof(S) < 2147483648.0;
+        const dim3 grid((row_tiles * blocks + kXcds - 1) / kXcds * kXcds);
+#define CIE_UP_OF(STEPS, EVEN)                                                                                                    \
+    adapter_up_strips<T, S, STEPS, EVEN><<<grid, kThreads, 0, s>>>(h, plan.parts, plan.chunks(k), up, scale, adapter, into, ld_into, out,    \
+                                                                   ld_out, rows, inner, n, rank, adapters, pieces, plan.block,           \
+                                                                   static_cast<int>(row_tiles), blocks, wide && near)
+#define CIE_UP(STEPS)                            \
+    if (rank % Operand<T>::kLane == 0)           \
+        CIE_UP_OF(STEPS, true);                  \
+    else if constexpr (Operand<T>::kLane > 4)    \
+    CIE_UP_OF(STEPS, false)
+        if (rank <= kStep) {
             CIE_UP(1);
-        else if (rank <= 2 * kStep)
+        } else if (rank <= 2 * kStep) {
             CIE_UP(2);
-        else if constexpr (kStep * 2 < 64)
+        } else if constexpr (kStep * 2 < 64) {
             CIE_UP(4);
+        }
 #undef CIE_UP
+#undef CIE_UP_OF
     }
     return cie_after_launch();
 }

@@ -1582,7 +1582,7 @@ def plan_lora(rows: int, k: int, n: int, inner: int, rank: int, count: int, shar
     chunk = max(1, -(-k // (32 * share))) * 2 * share
     chunks = -(-k // chunk)
     parts = chunks if rows * inner * chunks <= 1 << 20 else -(-chunks // 4)
-    tile_rows = 64 if rows <= 128 else 16
+    tile_rows = 64 if rows <= 128 or -(-rows // 64) * -(-inner // 64) * parts >= units else 16
     slots = min(count, rows, 16 if rows <= 128 else 2)
     tiles, strips = -(-rows // 64), -(-n // 128)
     many = tiles * strips >= 4 * units and rank <= 64
