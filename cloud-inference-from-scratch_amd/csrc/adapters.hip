@@ -156,7 +156,7 @@ __device__ __forceinline__ void down_rows(const Gathered& g, const T* __restrict
         for (int c = 0; c < C; ++c) acc[i][c] = quad_t{0.f, 0.f, 0.f, 0.f};
     }
     // a round is U steps of every wave; the next round is under way while one is multiplied, also across the end of a chunk
-    constexpr int U = R == 1 ? 2 : 1, kRound = kStep * kWaves * U;
+    constexpr int U = 2, kRound = kStep * kWaves * U;
     const int rounds = (k_end - k_begin + kRound - 1) / kRound, rounds_of_chunk = chunk / kRound;
     typename Op::type a[U][R], b[U][C];
     const auto ask = [&](int round) {
