@@ -88,13 +88,35 @@ __device__ __forceinline__ u64 last_lane(u64 v) {
                   __builtin_amdgcn_readlane(static_cast<int>(v >> 32), kWave - 1));
 }
 __device__ __forceinline__ u64 wave_sum_u64(u64 v) { return last_lane(wave_running_u64(v)); }
+// (0 is no number's better)
+__device__ __forceinline__ u64 larger(u64 a, u64 b) { return a > b ? a : b; }
 __device__ __forceinline__ u64 wave_most_u64(u64 v) {
-#pragma unroll
-    for (int offset = kWave / 2; offset > 0; offset >>= 1) {
-        const u64 other = __shfl_xor(v, offset, kWave);
-        v = other > v ? other : v;
+    v = larger(v, moved<0x111, 0xf>(v));
+    v = larger(v, moved<0x112, 0xf>(v));
+    v = larger(v, moved<0x114, 0xf>(v));
+    v = larger(v, moved<0x118, 0xf>(v));
+    v = larger(v, moved<0x142, 0xa>(v));
+    return last_lane(larger(v, moved<0x143, 0xc>(v)));
+}
+// A lane's partner, N (a power of two) lanes off by exclusive or.
+template <int N>
+__device__ __forceinline__ uint32_t partner(uint32_t v) {
+    if constexpr (N == 16) {
+        const swap_pair_t both = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return both[0] ^ both[1] ^ v;
+    } else if constexpr (N == 32) {
+        const swap_pair_t both = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return both[0] ^ both[1] ^ v;
+    } else if constexpr (N == 4) {  // 7 (a half row mirrored), then 3 (quads mirrored)
+        const int half = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x141, 0xf, 0xf, true);
+        return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, half, 0x1b, 0xf, 0xf, true));
+    } else {  // quads, or a row turned by half
+        return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), N == 1 ? 0xb1 : N == 2 ? 0x4e : 0x128, 0xf, 0xf, true));
     }
-    return v;
+}
+template <int N>
+__device__ __forceinline__ u64 partner_u64(u64 v) {
+    return joined(partner<N>(static_cast<uint32_t>(v)), partner<N>(static_cast<uint32_t>(v >> 32)));
 }
 
 // What the waves of a workgroup left in `s` (kCount of them): the sum of those in front of this one, and of all.
@@ -294,8 +316,11 @@ constexpr int kList = 4096;
 constexpr int kMaxParts = 2048;
 
 struct PartOf {
-    u64* best;       // [rows, parts] order << 32 | (0x7fffffff - index) of the largest
-    double* sum;     // [rows, parts] sum of exp((l - the part's largest) / T), where the row asks for it
+    struct Largest {
+        u64 best;    // order << 32 | (0x7fffffff - index)
+        double sum;  // of exp((l - the part's largest) / T), where the row asks for it
+    };
+    Largest* part;   // [rows, parts]
     float* chunk;    // [rows, parts * kPartThreads] the largest of each thread's 16; -inf where there is none
     // of rows under top-p or min-p without top-k:
     u64* kept;       // [rows, parts] weight of what lies in front of the cut's bin
@@ -370,7 +395,8 @@ rules_parts_kernel(const float* __restrict__ logits, const float* __restrict__ t
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kPartWaves; ++w) best = s_best[w] > best ? s_best[w] : best;
-    if (threadIdx.x == 0) of.best[static_cast<size_t>(r) * gridDim.x + part] = best;
+    PartOf::Largest* const mine = of.part + static_cast<size_t>(r) * gridDim.x + part;
+    if (threadIdx.x == 0) mine->best = best;
     const Rules rules(temperature, top_k, top_p, min_p, r, vocab);
     if (!rules.shares()) return;
     if (rules.tallied()) {  // (the launches behind this one add to them)
@@ -391,7 +417,7 @@ rules_parts_kernel(const float* __restrict__ logits, const float* __restrict__ t
     if (threadIdx.x == 0) {
         sum = 0.0;
         for (int w = 0; w < kPartWaves; ++w) sum += s_sum[w];
-        of.sum[static_cast<size_t>(r) * gridDim.x + part] = sum;
+        mine->sum = sum;
     }
 }
 
@@ -402,25 +428,30 @@ struct Whole {
     u64 best[kBlockWaves];
     double sum[kMaxParts];  // what each part weighs
 
-    __device__ __forceinline__ u64 find_best(const u64* part_best, int parts) {
+    __device__ __forceinline__ u64 find_best(const PartOf::Largest* part, int parts) {
         u64 found = 0;
-        for (int q = threadIdx.x; q < parts; q += kBlock) found = part_best[q] > found ? part_best[q] : found;
+        for (int q = threadIdx.x; q < parts; q += kBlock) found = larger(found, part[q].best);
         found = wave_most_u64(found);
         if (threadIdx.x % kWave == 0) best[threadIdx.x / kWave] = found;
         __syncthreads();
         return wave_most_u64(best[threadIdx.x % kBlockWaves]);
     }
     // (every wave the same: lanes take the parts in turn, and are added in one order)
-    __device__ __forceinline__ double find_total(const Row& row, const u64* part_best, const double* part_sum, int parts) {
+    __device__ __forceinline__ double find_total(const Row& row, const PartOf::Largest* part, int parts) {
         for (int q = threadIdx.x; q < parts; q += kBlock) {
-            const uint32_t key = static_cast<uint32_t>(part_best[q] >> 32);
-            sum[q] = key > kOrderOfMinusInf ? part_sum[q] * row.share(logit_of(key)) : 0.0;
+            const uint32_t key = static_cast<uint32_t>(part[q].best >> 32);
+            sum[q] = key > kOrderOfMinusInf ? part[q].sum * row.share(logit_of(key)) : 0.0;
         }
         __syncthreads();
         double total = 0.0;
         for (int q = threadIdx.x % kWave; q < parts; q += kWave) total += sum[q];
-#pragma unroll
-        for (int offset = kWave / 2; offset > 0; offset >>= 1) total += __shfl_xor(total, offset, kWave);
+        const auto with = [&](u64 other) { total += __builtin_bit_cast(double, other); };
+        with(partner_u64<1>(__builtin_bit_cast(u64, total)));
+        with(partner_u64<2>(__builtin_bit_cast(u64, total)));
+        with(partner_u64<4>(__builtin_bit_cast(u64, total)));
+        with(partner_u64<8>(__builtin_bit_cast(u64, total)));
+        with(partner_u64<16>(__builtin_bit_cast(u64, total)));
+        with(partner_u64<32>(__builtin_bit_cast(u64, total)));
         return total;
     }
 };
@@ -429,21 +460,21 @@ struct Whole {
 // What weighs less than (1 - p) / vocab of the sum, or less than m, is not kept however the rest is shared out.
 struct Reach {
     float best;
-    double distance;
+    double distance, bins;  // (and how many bins of the histogram a unit of distance has: they share the reach evenly)
     __device__ __forceinline__ Reach(const Row& row, const Rules& rules, double total) {
         best = row.best;
         const double least = rules.p < 1.0 ? fmax((1.0 - rules.p) * total / row.vocab, rules.m) : rules.m;
         distance = -log(least) * static_cast<double>(rules.temp) * (1.0 + 1e-9) + 1e-30;  // (a little rounded up)
+        bins = (kBins - 1) / distance;
     }
     __device__ __forceinline__ bool operator()(float l) const {
         return l > -INFINITY && (l == best || static_cast<double>(best) - static_cast<double>(l) <= distance);
     }
 };
 
-// The larger the nearer to the largest.  64 bins to a factor of e; all beyond e^-32 are one, where 8 million tokens together
-// weigh less than the least 1 - p that a float has.
-__device__ __forceinline__ int bin_of(const Row& row, float l) {
-    const double at = l == row.best ? 0.0 : (static_cast<double>(row.best) - static_cast<double>(l)) * row.inv_t * 64.0;
+// The larger the nearer to the largest.
+__device__ __forceinline__ int bin_of(const Reach& reach, float l) {
+    const double at = l == reach.best ? 0.0 : (static_cast<double>(reach.best) - static_cast<double>(l)) * reach.bins;
     return kBins - 1 - (at < kBins - 1 ? static_cast<int>(at) : kBins - 1);
 }
 
@@ -485,16 +516,16 @@ rules_tally_kernel(const float* __restrict__ logits, const float* __restrict__ t
     const int r = blockIdx.y;
     const Rules rules(temperature, top_k, top_p, min_p, r, vocab);
     if (!rules.tallied() || !(rules.p < 1.0)) return;
-    const u64* part_best = of.best + static_cast<size_t>(r) * parts;
+    const PartOf::Largest* of_parts = of.part + static_cast<size_t>(r) * parts;
     for (int b = threadIdx.x; b < kBins; b += kPartThreads) s_weight[b] = 0;
-    const uint32_t key = static_cast<uint32_t>(whole.find_best(part_best, parts) >> 32);
+    const uint32_t key = static_cast<uint32_t>(whole.find_best(of_parts, parts) >> 32);
     if (key <= kOrderOfMinusInf) return;
     const Row row = {logits + static_cast<size_t>(r) * ld, vocab, logit_of(key), 1.0 / static_cast<double>(rules.temp), unit, 0.0};
-    const Reach reach(row, rules, whole.find_total(row, part_best, of.sum + static_cast<size_t>(r) * parts, parts));
+    const Reach reach(row, rules, whole.find_total(row, of_parts, parts));
     for (int part = blockIdx.x; part < parts; part += gridDim.x)
         walk_chunk(row, of.chunk + static_cast<size_t>(r) * parts * kPartThreads, part, reach, [&](float l, int) {
             const u64 w = row.weight(l);
-            if (w) atomicAdd(&s_weight[bin_of(row, l)], w);
+            if (w) atomicAdd(&s_weight[bin_of(reach, l)], w);
         });
     __syncthreads();
     for (int b = threadIdx.x; b < kBins; b += kPartThreads)
@@ -513,15 +544,15 @@ rules_collect_kernel(const float* __restrict__ logits, const float* __restrict__
     const int r = blockIdx.y, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const Rules rules(temperature, top_k, top_p, min_p, r, vocab);
     if (!rules.tallied()) return;
-    const u64* part_best = of.best + static_cast<size_t>(r) * parts;
+    const PartOf::Largest* of_parts = of.part + static_cast<size_t>(r) * parts;
     if (threadIdx.x == 0) {
         s_bin = -1;
         s_above = 0;
     }
-    const uint32_t key = static_cast<uint32_t>(whole.find_best(part_best, parts) >> 32);
+    const uint32_t key = static_cast<uint32_t>(whole.find_best(of_parts, parts) >> 32);
     if (key <= kOrderOfMinusInf) return;
     const Row row = {logits + static_cast<size_t>(r) * ld, vocab, logit_of(key), 1.0 / static_cast<double>(rules.temp), unit, 0.0};
-    const double total = whole.find_total(row, part_best, of.sum + static_cast<size_t>(r) * parts, parts);
+    const double total = whole.find_total(row, of_parts, parts);
     const Reach reach(row, rules, total);
     if (rules.p < 1.0) {
         // the bin in which p of the weight is reached (without any, the lowest that has weight), and what lies in front of it
@@ -558,7 +589,7 @@ rules_collect_kernel(const float* __restrict__ logits, const float* __restrict__
         __syncthreads();
         u64 sum = 0;
         walk_chunk(row, of.chunk + static_cast<size_t>(r) * parts * kPartThreads, part, reach, [&](float l, int i) {
-            const int bin = bin_of(row, l);
+            const int bin = bin_of(reach, l);
             if (bin < cut_bin) return;
             const u64 w = row.weight(l);
             if (w == 0) return;
@@ -585,56 +616,96 @@ rules_collect_kernel(const float* __restrict__ logits, const float* __restrict__
 }
 
 // ---------------------------------------------------------------- last launch
-// list[0 .. n) in ascending order; n up to kList, the list's room up to the next power of two is written.  A thread holds kOwn
-// neighbours: numbers that are compared lie in one thread, in one wave, or pass through LDS.
+// The steps of a sorting network in which a wave's numbers, kOwn neighbours of each lane, are compared with those kApart places on and
+// then half as far each time, down to the next one: in registers.  (Written out: a loop's branches took longer than its steps.)
+template <int kOwn, int kApart>
+__device__ __forceinline__ void merge_steps(uint32_t (&own)[kOwn], int first, int run) {
+    uint32_t other[kOwn];
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+        if constexpr (kApart < kOwn)
+            other[i] = own[i ^ kApart];
+        else
+            other[i] = partner<kApart / kOwn>(own[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+        const bool smaller = (((first + i) & kApart) == 0) == (((first + i) & run) == 0);
+        own[i] = smaller ? min(own[i], other[i]) : max(own[i], other[i]);
+    }
+    if constexpr (kApart > 1) merge_steps<kOwn, kApart / 2>(own, first, run);
+}
+template <int kOwn, int kRun>
+__device__ __forceinline__ void sort_steps(uint32_t (&own)[kOwn], int first) {
+    merge_steps<kOwn, kRun / 2>(own, first, kRun);
+    if constexpr (kRun < kOwn * kWave) sort_steps<kOwn, kRun * 2>(own, first);
+}
+
+// keys[0 .. n) in ascending order; n up to kList, the room up to the next power of two (64 at least) is written.  Runs longer than a
+// wave's numbers pass through LDS until they are not.  (Orders alone: equal logits are told apart by their index only at the cut.)
 template <int kOwn>
-__device__ void sort_held(u64* list, int n, int size) {
-    u64 own[kOwn];
+__device__ void sort_held(uint32_t* keys, int n, int size) {
+    uint32_t own[kOwn];
     const int first = threadIdx.x * kOwn;
+    const bool idle = threadIdx.x / kWave * kWave * kOwn >= size;  // (a wave without numbers)
+    if (!idle) {
 #pragma unroll
-    for (int i = 0; i < kOwn; ++i) own[i] = first + i < n ? list[first + i] : ~0ull;
-    for (int run = 2; run <= size; run <<= 1) {
-        for (int apart = run >> 1; apart > 0; apart >>= 1) {
-            u64 other[kOwn];
-            if (apart >= kOwn * kWave) {
-                __syncthreads();
+        for (int i = 0; i < kOwn; ++i) own[i] = first + i < n ? keys[first + i] : ~0u;
+        sort_steps<kOwn, 2>(own, first);
+    }
+    for (int run = 2 * kOwn * kWave; run <= size; run <<= 1) {
+        for (int apart = run >> 1; apart >= kOwn * kWave; apart >>= 1) {
+            __syncthreads();
+            if (!idle) {
 #pragma unroll
-                for (int i = 0; i < kOwn; ++i)
-                    if (first + i < size) list[first + i] = own[i];
-                __syncthreads();
-#pragma unroll
-                for (int i = 0; i < kOwn; ++i) other[i] = first + i < size ? list[(first + i) ^ apart] : ~0ull;
-            } else if (apart >= kOwn) {
-#pragma unroll
-                for (int i = 0; i < kOwn; ++i) other[i] = __shfl_xor(own[i], apart / kOwn, kWave);
-            } else {
-#pragma unroll
-                for (int i = 0; i < kOwn; ++i) other[i] = apart == 1 ? own[i ^ 1] : own[(i ^ 2) % kOwn];
+                for (int i = 0; i < kOwn; ++i) keys[first + i] = own[i];
             }
+            __syncthreads();
+            if (!idle) {
 #pragma unroll
-            for (int i = 0; i < kOwn; ++i) {
-                const int at = first + i;
-                const bool low = (at & apart) == 0, up = (at & run) == 0;
-                if ((own[i] > other[i]) == (low == up)) own[i] = other[i];
+                for (int i = 0; i < kOwn; ++i) {
+                    const uint32_t other = keys[(first + i) ^ apart];
+                    const bool smaller = (((first + i) & apart) == 0) == (((first + i) & run) == 0);
+                    own[i] = smaller ? min(own[i], other) : max(own[i], other);
+                }
             }
         }
+        if (!idle) merge_steps<kOwn, kOwn * kWave / 2>(own, first, run);
     }
     __syncthreads();
+    if (!idle) {
 #pragma unroll
-    for (int i = 0; i < kOwn; ++i)
-        if (first + i < size) list[first + i] = own[i];
+        for (int i = 0; i < kOwn; ++i) keys[first + i] = own[i];
+    }
     __syncthreads();
 }
-__device__ void sort_list(u64* list, int n) {
-    int size = 2;
+__device__ void sort_keys(uint32_t* keys, int n) {
+    int size = kWave;
     while (size < n) size <<= 1;
     __syncthreads();
     if (size <= kThreads)
-        sort_held<1>(list, n, size);
+        sort_held<1>(keys, n, size);
     else if (size <= 2 * kThreads)
-        sort_held<2>(list, n, size);
+        sort_held<2>(keys, n, size);
     else
-        sort_held<4>(list, n, size);
+        sort_held<4>(keys, n, size);
+}
+
+// One wave's 64 numbers in ascending order.
+template <int kRun, int kApart>
+__device__ __forceinline__ void wave_sort_steps(u64& v) {
+    const int lane = threadIdx.x % kWave;
+    const u64 other = partner_u64<kApart>(v);
+    const bool smaller = ((lane & kApart) == 0) == ((lane & kRun) == 0);
+    v = (other < v) == smaller ? other : v;
+    if constexpr (kApart > 1)
+        wave_sort_steps<kRun, kApart / 2>(v);
+    else if constexpr (kRun < kWave)
+        wave_sort_steps<kRun * 2, kRun>(v);
+}
+__device__ __forceinline__ u64 wave_sort(u64 v) {
+    wave_sort_steps<2, 1>(v);
+    return v;
 }
 
 // Running sums in front of places: thread t has kPlaces of them, from t * kPlaces on.
@@ -672,48 +743,43 @@ struct Shared {
     union {
         Histogram h;
         int hits[kList];             // chunks that pass
-        u64 weight[kThreads / 4];    // of a short list
-        u64 segment[kMaxParts];      // of the parts
+        struct {
+            u64 segment[kMaxParts];  // the parts' weight
+            uint32_t keys[kList];    // of the list, by size
+        } cut;
     };
     union {
         u64 list[kList];
         Whole<kThreads> whole;
     };
     u64 sum[kWaves];
-    int count, hit_count, picked[kWaves], last[kWaves];
+    int count, hit_count;
 };
 
-// The smallest of the threads' first choices (0x7fffffff: none), the largest of their second ones (-1) if there is none.
+// The smallest of the threads' first choices (kNone: none), the largest of their second ones (-1) if there is none.
+constexpr int kNone = 0x7fffffff;
 __device__ __forceinline__ int choose(int first, int second, Shared& s) {
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const auto least = [](int v) {
-#pragma unroll
-        for (int offset = kWave / 2; offset > 0; offset >>= 1) v = min(v, __shfl_xor(v, offset, kWave));
-        return v;
-    };
-    first = least(first);
-    second = ~least(~second);
-    if (lane == 0) {
-        s.picked[wave] = first;
-        s.last[wave] = second;
-    }
+    // one number for both: a first choice counts more than any second one, and more the smaller it is
+    u64 mine = first != kNone ? (1ull << 32) + static_cast<uint32_t>(kNone - first) : static_cast<uint32_t>(second + 1);
+    mine = wave_most_u64(mine);
     __syncthreads();
-    first = least(s.picked[lane % kWaves]);
-    second = ~least(~s.last[lane % kWaves]);
+    if (lane == 0) s.sum[wave] = mine;
     __syncthreads();
-    return first != 0x7fffffff ? first : second;
+    mine = wave_most_u64(s.sum[lane % kWaves]);
+    return mine >> 32 ? kNone - static_cast<int>(mine & 0xffffffffu) : static_cast<int>(mine) - 1;
 }
 
 // The place whose running sum passes the target, of thread t's kPlaces from t * kPlaces on (`front` in front of them); the last
 // with any weight if none does, -1 without any.
 __device__ __forceinline__ int pick_place(const u64 (&own)[kPlaces], u64 front, double target, Shared& s) {
-    int mine = 0x7fffffff, last = -1;
+    int mine = kNone, last = -1;
 #pragma unroll
     for (int i = 0; i < kPlaces; ++i) {
         if (own[i] == 0) continue;
         last = threadIdx.x * kPlaces + i;
         front += own[i];
-        if (mine == 0x7fffffff && static_cast<double>(front) > target) mine = last;
+        if (mine == kNone && static_cast<double>(front) > target) mine = last;
     }
     return choose(mine, last, s);
 }
@@ -733,84 +799,118 @@ __device__ int draw_from_part(const Row& row, Shared& s, int part, u64 before, d
     return place < 0 ? -1 : part * kPart + place;
 }
 
-// The draw from a list of up to kThreads / 4 numbers that holds the first of the row's order, the first k of them, p, m and u: four
-// threads compare a number with all others, for its rank and what lies in front of it, then for the sum up to its index.
-__device__ int draw_from_few(const Row& row, Shared& s, int n, const Rules& rules, double u) {
-    const int i = threadIdx.x / 4, lane = threadIdx.x % 4;
-    const u64 mine = i < n ? s.list[i] : ~0ull;
-    const float l = logit_of(~static_cast<uint32_t>(mine >> 32));
-    const double share = i < n ? row.share(l) : 0.0;
-    u64 weight = static_cast<u64>(share * row.unit + 0.5);
-    __syncthreads();  // (the histogram and the hits lie where the weights go)
-    if (lane == 0) s.weight[i] = weight;
-    __syncthreads();
-    int rank = 0;
-    u64 front = 0;
-    for (int j = lane; j < n; j += 4)
-        if (s.list[j] < mine) {
-            ++rank;
-            front += s.weight[j];
+// The part in which the running sum of s.cut.segment passes u times the whole, and its draw.  (A part whose numbers each round to no
+// weight, though their sum has one, has nothing to draw: the next one then.)
+__device__ int draw_from_segments(const Row& row, Shared& s, int parts, double u, u64 cut) {
+    // every wave the same
+    const int lane = threadIdx.x % kWave;
+    u64 all = 0;
+    for (int q = lane; q < parts; q += kWave) all += s.cut.segment[q];
+    const double target = u * static_cast<double>(wave_sum_u64(all));
+    int owner = 0;
+    u64 before = 0, running = 0;
+    for (int base = 0; base < parts; base += kWave) {
+        const u64 own = base + lane < parts ? s.cut.segment[base + lane] : 0;
+        const u64 sum = running + wave_running_u64(own);
+        const u64 passed = __ballot(own && static_cast<double>(sum) > target), any = __ballot(own > 0);
+        if (any) {
+            const int which = passed ? __ffsll(passed) - 1 : 63 - __clzll(any);
+            owner = base + which;
+            const u64 front = sum - own;
+            before = joined(__builtin_amdgcn_readlane(static_cast<int>(front & 0xffffffffu), which),
+                            __builtin_amdgcn_readlane(static_cast<int>(front >> 32), which));
         }
-#pragma unroll
-    for (int offset = 1; offset < 4; offset <<= 1) {
-        rank += __shfl_xor(rank, offset, kWave);
-        front += __shfl_xor(front, offset, kWave);
+        if (passed) break;
+        running = last_lane(sum);
     }
-    bool kept = i < n && rank < rules.k;
-    if (rules.p < 1.0) {
-        const double limit = rules.p * static_cast<double>(block_sum_u64(kept && lane == 0 ? weight : 0, s.sum));
-        kept = kept && (rank == 0 || static_cast<double>(front) < limit);
-    }
-    kept = kept && (rank == 0 || !(rules.m > 0.0) || share >= rules.m);
-    if (!kept) weight = 0;
-    const double target = u * static_cast<double>(block_sum_u64(lane == 0 ? weight : 0, s.sum));
-    if (lane == 0) s.weight[i] = weight;  // (all have read the old ones: the sum has barriers)
-    __syncthreads();
-    const uint32_t index = static_cast<uint32_t>(mine);
-    u64 running = 0;
-    for (int j = lane; j < n; j += 4)
-        if (static_cast<uint32_t>(s.list[j]) <= index) running += s.weight[j];
-#pragma unroll
-    for (int offset = 1; offset < 4; offset <<= 1) running += __shfl_xor(running, offset, kWave);
-    return choose(weight && static_cast<double>(running) > target ? static_cast<int>(index) : 0x7fffffff,
-                  weight ? static_cast<int>(index) : -1, s);
+    int picked = draw_from_part(row, s, owner, before, target, cut);
+    for (int q = owner + 1; q < parts && picked < 0; ++q) picked = draw_from_part(row, s, q, 0, -1.0, cut);
+    return picked;
 }
 
-// ... from a longer one.
-__device__ int draw_from_list(const Row& row, Shared& s, int n, const Rules& rules, double u) {
-    sort_list(s.list, n);
-    n = min(n, rules.k);
+// Which of a wave's weights, in the order of the lanes, passes u times their sum: its lane, or the last with any weight, or -1.
+__device__ __forceinline__ int pick_lane(u64 weight, double u) {
+    const u64 running = wave_running_u64(weight);
+    const double target = u * static_cast<double>(last_lane(running));
+    const u64 passed = __ballot(weight && static_cast<double>(running) > target), any = __ballot(weight > 0);
+    return passed ? __ffsll(passed) - 1 : any ? 63 - __clzll(any) : -1;
+}
+
+// The cut of a list: of its n numbers by size the first k, of these the ones in front of which less than `limit` lies (p of what
+// the k weigh, of_list; `above` lies in front of the list), of these the ones that weigh at least m (but never none).  The last
+// kept place comes back (all threads; `front` of nothing: none is kept only with something above).
+__device__ u64 cut_list(const Row& row, Shared& s, int n, int k, bool nucleus, bool of_list, double p_or_limit, double m, u64 above) {
+    for (int i = threadIdx.x; i < n; i += kThreads) s.cut.keys[i] = static_cast<uint32_t>(s.list[i] >> 32);
+    sort_keys(s.cut.keys, n);
+    const int count = min(n, k), first = threadIdx.x * kPlaces;
     u64 own[kPlaces], total;
-    const int first = threadIdx.x * kPlaces;
 #pragma unroll
-    for (int i = 0; i < kPlaces; ++i)
-        own[i] = first + i < n ? row.weight(logit_of(~static_cast<uint32_t>(s.list[first + i] >> 32))) : 0;
-    u64 front = sums_in_front(own, s.sum, total);
-    const double limit = rules.p * static_cast<double>(total);
-    int kept = 0;  // (what is kept is a prefix of all places, so the threads' numbers add up to it)
+    for (int i = 0; i < kPlaces; ++i) own[i] = first + i < count ? row.weight(logit_of(~s.cut.keys[first + i])) : 0;
+    u64 front = above + sums_in_front(own, s.sum, total);
+    const double limit = of_list ? p_or_limit * static_cast<double>(total) : p_or_limit;
+    int mine = 0;  // (what is kept is a prefix of all places, so the threads' numbers add up to it)
 #pragma unroll
     for (int i = 0; i < kPlaces; ++i) {
-        if (first + i >= n) continue;
-        const bool in_p = first + i == 0 || !(rules.p < 1.0) || static_cast<double>(front) < limit;
-        const bool in_m = first + i == 0 || !(rules.m > 0.0) || row.share(logit_of(~static_cast<uint32_t>(s.list[first + i] >> 32))) >= rules.m;
-        kept += in_p && in_m;
+        if (first + i >= count) continue;
+        const bool very_first = first + i == 0 && above == 0;
+        const bool in_p = very_first || !nucleus || static_cast<double>(front) < limit;
+        const bool in_m = very_first || !(m > 0.0) || row.share(logit_of(~s.cut.keys[first + i])) >= m;
+        mine += in_p && in_m;
         front += own[i];
     }
-    n = static_cast<int>(block_sum_u64(kept, s.sum));
-    // the kept ones by index, their logits' order beside it
-    u64 turned[kPlaces];
-#pragma unroll
-    for (int i = 0; i < kPlaces; ++i) turned[i] = first + i < n ? s.list[first + i] << 32 | s.list[first + i] >> 32 : 0;
+    const int kept = static_cast<int>(block_sum_u64(mine, s.sum));
+    if (kept == 0) return (static_cast<u64>(s.cut.keys[0]) << 32) - 1;
+    // of the numbers equal to the last kept one only the first by index, if not all
+    const uint32_t key = s.cut.keys[kept - 1];
+    u64 counts = 0;  // the larger ones, and the equal ones
+    for (int i = threadIdx.x; i < n; i += kThreads) counts += s.cut.keys[i] < key ? 1ull : s.cut.keys[i] == key ? 1ull << 32 : 0;
+    counts = block_sum_u64(counts, s.sum);
+    const int equal = static_cast<int>(counts >> 32), wanted = kept - static_cast<int>(counts & 0xffffffffu);
+    if (wanted >= equal) return (static_cast<u64>(key) << 32) | 0xffffffffu;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kPlaces; ++i)
-        if (first + i < n) s.list[first + i] = turned[i];
-    sort_list(s.list, n);
-#pragma unroll
-    for (int i = 0; i < kPlaces; ++i) own[i] = first + i < n ? row.weight(logit_of(~static_cast<uint32_t>(s.list[first + i]))) : 0;
-    front = sums_in_front(own, s.sum, total);
-    const int place = pick_place(own, front, u * static_cast<double>(total), s);
-    return place < 0 ? -1 : static_cast<int>(s.list[place] >> 32);
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const u64 place = s.list[i];
+        if (static_cast<uint32_t>(place >> 32) != key) continue;
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += s.list[j] < place && static_cast<uint32_t>(s.list[j] >> 32) == key;
+        if (rank == wanted - 1) s.sum[0] = place;
+    }
+    __syncthreads();
+    const u64 cut = s.sum[0];
+    __syncthreads();
+    return cut;
+}
+
+// The draw from a list that holds the first of the row's order.
+__device__ int draw_from_list(const Row& row, Shared& s, int n, int parts, const Rules& rules, double u) {
+    if (n <= kWave) {  // one wave, a number to a lane: without a barrier
+        if (threadIdx.x < kWave) {
+            const int lane = threadIdx.x;
+            const u64 place = wave_sort(lane < n ? s.list[lane] : ~0ull);
+            const float l = logit_of(~static_cast<uint32_t>(place >> 32));
+            const double share = lane < min(n, rules.k) ? row.share(l) : 0.0;
+            u64 weight = static_cast<u64>(share * row.unit + 0.5);
+            const u64 running = wave_running_u64(weight);
+            const double limit = rules.p * static_cast<double>(last_lane(running));
+            if (lane > 0 && ((rules.p < 1.0 && !(static_cast<double>(running - weight) < limit)) || (rules.m > 0.0 && share < rules.m))) weight = 0;
+            const u64 kept = wave_sort(weight ? place << 32 | place >> 32 : ~0ull);  // by index
+            weight = kept != ~0ull ? row.weight(logit_of(~static_cast<uint32_t>(kept))) : 0;
+            const int which = pick_lane(weight, u);
+            if (lane == max(0, which)) s.count = which < 0 ? -1 : static_cast<int>(kept >> 32);
+        }
+        __syncthreads();
+        return s.count;
+    }
+    const u64 cut = cut_list(row, s, n, rules.k, rules.p < 1.0, true, rules.p, rules.m, 0);
+    // where the kept ones lie: the parts' sums
+    for (int q = threadIdx.x; q < parts; q += kThreads) s.cut.segment[q] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const u64 place = s.list[i];
+        if (place <= cut) atomicAdd(&s.cut.segment[static_cast<uint32_t>(place) / kPart], row.weight(logit_of(~static_cast<uint32_t>(place >> 32))));
+    }
+    __syncthreads();
+    return draw_from_segments(row, s, parts, u, cut);
 }
 
 // The draw under top-k; -2: too many numbers pass the bound.
@@ -880,36 +980,7 @@ __device__ int draw_of_k(const Row& row, Shared& s, const float* chunks, int chu
     __syncthreads();
     const int n = s.count;
     if (n > kList) return -2;
-    return n <= kThreads / 4 ? draw_from_few(row, s, n, rules, u) : draw_from_list(row, s, n, rules, u);
-}
-
-// The part in which the running sum of s.segment passes u times the whole, and its draw.  (A part whose numbers each round to no
-// weight, though their sum has one, has nothing to draw: the next one then.)
-__device__ int draw_from_segments(const Row& row, Shared& s, int parts, double u, u64 cut) {
-    // every wave the same
-    const int lane = threadIdx.x % kWave;
-    u64 all = 0;
-    for (int q = lane; q < parts; q += kWave) all += s.segment[q];
-    const double target = u * static_cast<double>(wave_sum_u64(all));
-    int owner = 0;
-    u64 before = 0, running = 0;
-    for (int base = 0; base < parts; base += kWave) {
-        const u64 own = base + lane < parts ? s.segment[base + lane] : 0;
-        const u64 sum = running + wave_running_u64(own);
-        const u64 passed = __ballot(own && static_cast<double>(sum) > target), any = __ballot(own > 0);
-        if (any) {
-            const int which = passed ? __ffsll(passed) - 1 : 63 - __clzll(any);
-            owner = base + which;
-            const u64 front = sum - own;
-            before = joined(__builtin_amdgcn_readlane(static_cast<int>(front & 0xffffffffu), which),
-                            __builtin_amdgcn_readlane(static_cast<int>(front >> 32), which));
-        }
-        if (passed) break;
-        running = last_lane(sum);
-    }
-    int picked = draw_from_part(row, s, owner, before, target, cut);
-    for (int q = owner + 1; q < parts && picked < 0; ++q) picked = draw_from_part(row, s, q, 0, -1.0, cut);
-    return picked;
+    return draw_from_list(row, s, n, chunk_count / kPartThreads, rules, u);
 }
 
 // The draw of a row that was tallied; -2: the cut's bin holds more than its list.
@@ -918,31 +989,18 @@ __device__ int draw_of_tally(Row& row, Shared& s, const PartOf& of, int r, int p
     if (rules.p < 1.0 && listed > kList) return -2;
     const int n = rules.p < 1.0 ? static_cast<int>(listed) : 0;
     const double limit = rules.p * total * row.unit;
-    for (int q = threadIdx.x; q < parts; q += kThreads) s.segment[q] = of.kept[static_cast<size_t>(r) * parts + q];
+    for (int q = threadIdx.x; q < parts; q += kThreads) s.cut.segment[q] = of.kept[static_cast<size_t>(r) * parts + q];
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += kThreads) s.list[i] = of.list[static_cast<size_t>(r) * kList + i];
     u64 cut = ~0ull;  // the last kept place
-    if (rules.p < 1.0) {
-        sort_list(s.list, n);
-        u64 own[kPlaces], weight;
-        const int first = threadIdx.x * kPlaces;
-#pragma unroll
-        for (int i = 0; i < kPlaces; ++i)
-            own[i] = first + i < n ? row.weight(logit_of(~static_cast<uint32_t>(s.list[first + i] >> 32))) : 0;
-        u64 front = above + sums_in_front(own, s.sum, weight);
-        int kept = 0;  // (a prefix of the places)
-#pragma unroll
-        for (int i = 0; i < kPlaces; ++i) {
-            if (first + i >= n || !(front == 0 || static_cast<double>(front) < limit)) continue;
-            front += own[i];
-            ++kept;
-            const u64 place = s.list[first + i];
-            if (own[i] && (!(rules.m > 0.0) || row.share(logit_of(~static_cast<uint32_t>(place >> 32))) >= rules.m))
-                atomicAdd(&s.segment[static_cast<uint32_t>(place) / kPart], own[i]);
+    if (n > 0) {
+        __syncthreads();
+        cut = cut_list(row, s, n, n, true, false, limit, rules.m, above);
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+            const u64 place = s.list[i];
+            if (place <= cut) atomicAdd(&s.cut.segment[static_cast<uint32_t>(place) / kPart], row.weight(logit_of(~static_cast<uint32_t>(place >> 32))));
         }
-        const int last = static_cast<int>(block_sum_u64(kept, s.sum));
-        // (nothing of the bin is kept only if rounding says so: the cut then lies right in front of it)
-        cut = last > 0 ? s.list[last - 1] : n > 0 ? s.list[0] - 1 : ~0ull;
+        __syncthreads();
     }
     row.least = rules.m;
     return draw_from_segments(row, s, parts, u, cut);
@@ -954,9 +1012,9 @@ rules_draw_kernel(const float* __restrict__ logits, const float* __restrict__ te
                   int* __restrict__ out, int vocab, long ld, int parts, double unit) {
     __shared__ Shared s;
     const int r = blockIdx.x;
-    const u64* part_best = of.best + static_cast<size_t>(r) * parts;
+    const PartOf::Largest* of_parts = of.part + static_cast<size_t>(r) * parts;
     const Rules rules(temperature, top_k, top_p, min_p, r, vocab);
-    const u64 best = s.whole.find_best(part_best, parts);
+    const u64 best = s.whole.find_best(of_parts, parts);
     const uint32_t best_key = static_cast<uint32_t>(best >> 32);
     const int best_idx = best_key > kOrderOfMinusInf ? 0x7fffffff - static_cast<int>(best & 0xffffffffu) : 0;
     if (!rules.draws() || best_key <= kOrderOfMinusInf) {
@@ -970,13 +1028,13 @@ rules_draw_kernel(const float* __restrict__ logits, const float* __restrict__ te
     if (rules.k > 0) {
         picked = draw_of_k(row, s, of.chunk + static_cast<size_t>(r) * parts * kPartThreads, parts * kPartThreads, rules, u);
     } else {
-        const double total = s.whole.find_total(row, part_best, of.sum + static_cast<size_t>(r) * parts, parts);
+        const double total = s.whole.find_total(row, of_parts, parts);
         if (rules.tallied()) {
             __syncthreads();
             picked = draw_of_tally(row, s, of, r, parts, rules, total, u);
         } else {
             __syncthreads();
-            for (int q = threadIdx.x; q < parts; q += kThreads) s.segment[q] = static_cast<u64>(s.whole.sum[q] * unit + 0.5);
+            for (int q = threadIdx.x; q < parts; q += kThreads) s.cut.segment[q] = static_cast<u64>(s.whole.sum[q] * unit + 0.5);
             __syncthreads();
             picked = draw_from_segments(row, s, parts, u, ~0ull);
         }
@@ -1005,9 +1063,8 @@ CIE_API int cie_sample_rules(void* stream, const float* logits, const float* tem
     const int parts = (vocab + kPart - 1) / kPart;
     const size_t all = static_cast<size_t>(rows) * parts;
     PartOf of;
-    of.best = static_cast<u64*>(work);
-    of.sum = reinterpret_cast<double*>(of.best + all);
-    of.kept = reinterpret_cast<u64*>(of.sum + all);
+    of.part = static_cast<PartOf::Largest*>(work);
+    of.kept = reinterpret_cast<u64*>(of.part + all);
     of.chunk = reinterpret_cast<float*>(of.kept + all);
     of.histogram = reinterpret_cast<u64*>(of.chunk + all * kPartThreads);
     of.list = of.histogram + static_cast<size_t>(rows) * kBins;
