@@ -1508,7 +1508,7 @@ def _per_row(name: str, t: torch.Tensor, dtype: torch.dtype, rows: int) -> None:
 MAX_RULE_ROWS, MAX_RULE_VOCAB = 65535, 1 << 23
 # The workspace of a draw under rules, in words of 8 bytes: for each part of so many logits, and for a row's histogram and list
 RULES_PART, RULES_PART_WORDS, RULES_ROW_WORDS = 4096, 131, 2048 + 4096 + 2
-RULES_SPREAD = 2048  # workgroups of a launch in which rows without top-p and min-p have nothing to do
+RULES_SPREAD = 2560  # workgroups of a launch in which rows without top-p and min-p have nothing to do
 
 
 def _sample_rules(logits, temperature, uniform, out, top_k, top_p, min_p) -> torch.Tensor:
