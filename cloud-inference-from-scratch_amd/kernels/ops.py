@@ -1489,13 +1489,22 @@ def _on_current_gpu(first: torch.Tensor, *others: Optional[torch.Tensor]) -> Non
             raise ValueError(f"operands on {first.device} and {other.device}")
 
 
-def _logit_rows(logits: torch.Tensor) -> tuple[int, int]:
-    """Float32 rows on the GPU, each in one piece (they may lie apart)."""
-    _row_view("logits", logits, tuple(logits.shape), (torch.float32,))
-    rows, vocab = logits.shape
-    if vocab < 1:
+def _rows_apart(name: str, t: torch.Tensor, rows: int, columns: int, dtype: torch.dtype) -> int:
+    """The distance of the rows of a GPU matrix [rows, columns], each in one piece."""
+    if t.dim() == 2 and t.shape == (rows, columns) and t.dtype is dtype and t.is_cuda:
+        apart, inner = t.stride()
+        if inner == 1 and (rows <= 1 or apart >= columns):
+            return apart if rows > 1 else max(apart, columns)
+    _row_view(name, t, (rows, columns), (dtype,))
+    return _ld(t)
+
+
+def _logit_rows(logits: torch.Tensor) -> tuple[int, int, int]:
+    """(rows, vocabulary, distance of the rows) of float32 logits on the GPU, each row in one piece."""
+    if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"logits of shape {tuple(logits.shape)}")
-    return rows, vocab
+    rows, vocab = logits.shape
+    return rows, vocab, _rows_apart("logits", logits, rows, vocab, torch.float32)
 
 
 def _per_row(name: str, t: torch.Tensor, dtype: torch.dtype, rows: int) -> None:
@@ -1512,7 +1521,7 @@ RULES_SPREAD = 2560  # workgroups of a launch in which rows without top-p and mi
 
 
 def _sample_rules(logits, temperature, uniform, out, top_k, top_p, min_p) -> torch.Tensor:
-    rows, vocab = _logit_rows(logits)
+    rows, vocab, apart = _logit_rows(logits)
     if temperature is None or uniform is None:
         raise ValueError("a draw under rules needs temperatures and uniform numbers")
     if rows > MAX_RULE_ROWS or vocab > MAX_RULE_VOCAB:
@@ -1529,16 +1538,16 @@ def _sample_rules(logits, temperature, uniform, out, top_k, top_p, min_p) -> tor
     if top_p is not None or min_p is not None:
         words += RULES_ROW_WORDS
     if out is None:
-        out = torch.empty((rows,), dtype=torch.int32, device=logits.device)
+        out = logits.new_empty((rows,), dtype=torch.int32)
     else:
         _per_row("out", out, torch.int32, rows)
     _on_current_gpu(logits, temperature, uniform, top_k, top_p, min_p, out)
     if rows == 0:
         return out
-    work = torch.empty((rows * words,), dtype=torch.int64, device=logits.device)
+    work = logits.new_empty((rows * words,), dtype=torch.int64)
     _run("cie_sample_rules", load_library().cie_sample_rules(
         _stream(), logits.data_ptr(), temperature.data_ptr(), uniform.data_ptr(), _ptr(top_k), _ptr(top_p), _ptr(min_p), out.data_ptr(),
-        work.data_ptr(), rows, vocab, _ld(logits), max(1, RULES_SPREAD // rows)))
+        work.data_ptr(), rows, vocab, apart, max(1, RULES_SPREAD // rows)))
     return out
 
 
@@ -1550,12 +1559,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, out: Optional[tor
     """What the rows of float32 logits give their tokens (int32 [rows]): ``(l_t - max l) - log sum_i exp(l_i - max l)``, float32
     [rows].  The rows of ``logits`` may lie apart.  A token outside the vocabulary gives NaN, and so does a row with a NaN, a
     +inf, or nothing but -inf."""
-    rows, vocab = _logit_rows(logits)
+    rows, vocab, apart = _logit_rows(logits)
     _per_row("tokens", tokens, torch.int32, rows)
     if rows > MAX_RULE_ROWS or vocab > 1 << 30:
         raise ValueError(f"up to {MAX_RULE_ROWS} rows of {1 << 30} logits, not {rows} of {vocab}")
     if out is None:
-        out = torch.empty((rows,), dtype=torch.float32, device=logits.device)
+        out = logits.new_empty((rows,))
     else:
         _per_row("out", out, torch.float32, rows)
     _on_current_gpu(logits, tokens, out)
@@ -1563,9 +1572,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, out: Optional[tor
         return out
     turns = -(-vocab // LOGPROB_TURN)
     part = -(-turns // min(turns, max(1, LOGPROB_SPREAD // rows))) * LOGPROB_TURN
-    tallies = None if part >= vocab else torch.empty(2 * rows * -(-vocab // part), dtype=torch.float32, device=logits.device)
+    tallies = None if part >= vocab else logits.new_empty((2 * rows * -(-vocab // part),))
     _run("cie_token_logprobs", load_library().cie_token_logprobs(
-        _stream(), _ptr(logits), _ptr(tokens), _ptr(tallies), _ptr(out), _i(rows), _i(vocab), _i(_ld(logits)), _i(part)))
+        _stream(), logits.data_ptr(), tokens.data_ptr(), _ptr(tallies), out.data_ptr(), rows, vocab, apart, part))
     return out
 
 
@@ -1607,8 +1616,10 @@ def lora_add(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale: torch
     n = into.shape[1]
     dtype, out_dtype = x.dtype, into.dtype
     code = _code(dtype)
-    _row_view("x", x, (rows, k), (dtype,))
-    _row_view("into", into, (rows, n), (dtype, torch.float32))
+    if out_dtype is not dtype and out_dtype is not torch.float32:
+        raise ValueError(f"into must be {dtype} or float32, is {out_dtype}")
+    ldx = _rows_apart("x", x, rows, k, dtype)
+    ld_into = _rows_apart("into", into, rows, n, out_dtype)
     columns = (n,) if columns is None else tuple(columns)
     pieces = len(columns)
     if not 1 <= pieces <= MAX_ADAPTER_PIECES or min(columns) < 1 or sum(columns) != n:
@@ -1621,27 +1632,27 @@ def lora_add(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale: torch
                          f"and a rank of 1 to {MAX_ADAPTER_RANK}")
     _per_row("scale", scale, torch.float32, count)
     _per_row("adapters", adapters, torch.int32, rows)
-    if out is None:
-        out = into
+    if out is None or out is into:
+        out, ld_out = into, ld_into
     else:
-        _row_view("out", out, (rows, n), (out_dtype,))
+        ld_out = _rows_apart("out", out, rows, n, out_dtype)
     _on_current_gpu(x, down, up, scale, adapters, into, out)
     if rows > 65535:
         raise ValueError(f"up to 65,535 rows, not {rows}")
     if rows == 0:
         return out
     size = 4 if code == F32 else 2
-    ldx, x_at, down_at, up_at = _ld(x), x.data_ptr(), down.data_ptr(), up.data_ptr()
+    x_at, down_at, up_at = x.data_ptr(), down.data_ptr(), up.data_ptr()
     if rank % 4 == 0 and (k * size | ldx * size | x_at | down_at | up_at) % 16 == 0:
         plan = plan_lora(rows, k, n, pieces * rank, rank, count, 256 // size, compute_units())
     else:  # (a rank or a row that 16-byte loads do not take)
         plan = (0, 0, 0, 0, 0, 0)
-    inner = torch.empty((max(1, plan[1]) * rows * pieces * rank,), dtype=torch.float32, device=x.device)
+    inner = x.new_empty((max(1, plan[1]) * rows * pieces * rank,), dtype=torch.float32)
     c1 = columns[0]
     c2 = c1 + columns[1] if pieces > 1 else n
     _run("cie_lora_add", load_library().cie_lora_add(
-        _stream(), code, _CODES[out_dtype], x_at, ldx, down_at, up_at, scale.data_ptr(), adapters.data_ptr(), into.data_ptr(), _ld(into),
-        out.data_ptr(), _ld(out), inner.data_ptr(), rows, k, n, rank, count, pieces, c1, c2, c2 + columns[2] if pieces > 2 else n, *plan))
+        _stream(), code, _CODES[out_dtype], x_at, ldx, down_at, up_at, scale.data_ptr(), adapters.data_ptr(), into.data_ptr(), ld_into,
+        out.data_ptr(), ld_out, inner.data_ptr(), rows, k, n, rank, count, pieces, c1, c2, c2 + columns[2] if pieces > 2 else n, *plan))
     return out
 
 
