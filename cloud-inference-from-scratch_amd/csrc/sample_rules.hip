@@ -333,7 +333,7 @@ constexpr int kPartThreads = 256;
 constexpr int kPart = kPartThreads * 16;  // numbers of a part: a thread has four times four neighbours, 1,024 numbers apart
 
 constexpr int kList = 4096;
-constexpr int kMaxParts = 2048;
+constexpr int kMaxParts = 1024;
 
 struct PartOf {
     struct Largest {

@@ -1514,7 +1514,7 @@ def _per_row(name: str, t: torch.Tensor, dtype: torch.dtype, rows: int) -> None:
     raise ValueError(f"{name} must be [{rows}], is {list(t.shape)}")
 
 
-MAX_RULE_ROWS, MAX_RULE_VOCAB = 65535, 1 << 23
+MAX_RULE_ROWS, MAX_RULE_VOCAB = 65535, 1 << 22
 # The workspace of a draw under rules, in words of 8 bytes: for each part of so many logits, and for a row's histogram and list
 RULES_PART, RULES_PART_WORDS, RULES_ROW_WORDS = 4096, 131, 2048 + 4096 + 2
 RULES_SPREAD = 2560  # workgroups of a launch in which rows without top-p and min-p have nothing to do
@@ -1636,6 +1636,8 @@ def lora_add(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale: torch
         out, ld_out = into, ld_into
     else:
         ld_out = _rows_apart("out", out, rows, n, out_dtype)
+        if ld_out != ld_into and out.data_ptr() == into.data_ptr():
+            raise ValueError("out lies where into does, with its rows at another distance")
     _on_current_gpu(x, down, up, scale, adapters, into, out)
     if rows > 65535:
         raise ValueError(f"up to 65,535 rows, not {rows}")
