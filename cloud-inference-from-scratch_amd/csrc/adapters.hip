@@ -9,6 +9,10 @@
 // taken in tiles of consecutive ones; what a tile does is done once for each adapter that its rows have, on these rows alone,
 // gathered into matrix-core tiles of 16.  So no plan of who has which adapter is made on the host, a row's sums do not depend
 // on its neighbours, and a prompt (one adapter) and 64 requests (16 of them) run through the same code.
+//
+// Measured, both products, with what has to be read and written: one row of 2,048 and 2,560 columns, rank 16: 8.0 us (0.3 MB); 64
+// rows of 16 adapters, 2,048 and 22,016, rank 16: 17 us (19 MB); 24 rows of 8, 18,944 and 3,584, rank 32: 12.5 us (11.5 MB);
+// 2,048 rows of two, 3,584 and 37,888, rank 64: 110 us (339 MB).
 #include "common.h"
 
 namespace {
@@ -127,7 +131,10 @@ __device__ __forceinline__ Gathered gather(int id, u64 left) {
 // `slots`-th of its tile's adapters.  K falls into chunks whose length depends on K alone; four waves share a chunk's k and join
 // their sums through LDS, chunks are added one after the other in groups of kGroup, and the groups one after the other.  A part is
 // one chunk (few rows: as many workgroups as there are) or a group of them (many rows: fewer sums to write and read): either
-// way h is the same sum in the same order, whatever rows are beside it.
+// way h is the same sum in the same order, whatever rows are beside it.  Few rows are bound by the way to their first result (one row
+// of 2,048 at rank 16 x 3: 4.0 us; 24 rows of 8 adapters, K 18,944: 6.5 us for 11 MB of weights); 2,048 rows of 3,584 at rank 64 x 2,
+// 22.6 us, by the waits of the one workgroup that each CU has (59 MB through L2: the rows for two column groups, the weights for
+// 32 row tiles; 83 TFLOP/s).  More workgroups would mean more parts to write and to add, which costs the second product more.
 template <typename T, int C, int R>
 __device__ __forceinline__ void down_rows(const Gathered& g, const T* __restrict__ x, long ldx, const T* __restrict__ down,
                                           float* __restrict__ part, int row0, int inner, int j0, int k, int k_begin, int k_end,
@@ -155,7 +162,7 @@ __device__ __forceinline__ void down_rows(const Gathered& g, const T* __restrict
 #pragma unroll
         for (int c = 0; c < C; ++c) acc[i][c] = quad_t{0.f, 0.f, 0.f, 0.f};
     }
-    // a round is U steps of every wave; the next round is under way while one is multiplied, also across the end of a chunk
+    // a round is U steps of every wave (U of 1: 2,048 rows 24 us, not 22); the next round is under way while one is multiplied, also across the end of a chunk
     constexpr int U = 2, kRound = kStep * kWaves * U;
     const int rounds = (k_end - k_begin + kRound - 1) / kRound, rounds_of_chunk = chunk / kRound;
     typename Op::type a[U][R], b[U][C];
@@ -313,92 +320,6 @@ __device__ __forceinline__ words_t Piece<bf16_t>::sum(words_t old, const float (
     return old;
 }
 
-// A wave's share of the second product: the rows of one adapter, 16 at a time, and a strip of columns.  h is the first operand,
-// the strip's columns the second, dealt to the instructions so that a lane's results are 16 bytes of neighbouring columns (in
-// four rows), and 16 lanes have 256 bytes of a row in one piece.
-template <typename T, typename S, int kSteps>
-struct Share {
-    typedef Operand<T> Op;
-    static constexpr int kOwn = Piece<S>::kNumbers, kStrip = kTile * kOwn;
-    typename Op::type weights[kSteps][kOwn];
-    words_t next[4];
-    const int* order;
-    int adapter, count, first;  // first: of the lane's columns
-    bool whole;
-
-    __device__ __forceinline__ void ask_rows(int begin, const S* into, long ld_into) {
-        const int quarter = threadIdx.x % kWave / kTile;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int which = begin + quarter * 4 + i;
-            if (whole && which < count) next[i] = *reinterpret_cast<const words_t*>(into + static_cast<size_t>(order[which]) * ld_into + first);
-        }
-    }
-
-    // (the rows: `count` of them in `order`)
-    __device__ __forceinline__ void ask(const int* order_, int count_, int adapter_, int c0, int end, const T* up, int n, int rank,
-                                        const S* into, long ld_into, bool wide) {
-        const int lane = threadIdx.x % kWave, quarter = lane / kTile;
-        order = order_;
-        count = count_;
-        adapter = adapter_;
-        first = c0 + lane % kTile * kOwn;
-        whole = wide && first + kOwn <= end;
-        if (adapter >= 0) {
-#pragma unroll
-            for (int j = 0; j < kOwn; ++j) {
-                const int c = first + j < end ? first + j : end - 1;
-                const T* from = up + (static_cast<size_t>(adapter) * n + c) * rank;
-#pragma unroll
-                for (int s = 0; s < kSteps; ++s) weights[s][j] = up_numbers(from, (s * kQuarters + quarter) * Op::kLane, rank);
-            }
-        }
-        ask_rows(0, into, ld_into);
-    }
-
-    template <typename H>
-    __device__ __forceinline__ void finish(const H& h, int end, const S* into, long ld_into, S* out, long ld_out) {
-        const int lane = threadIdx.x % kWave, quarter = lane / kTile;
-        for (int begin = 0; begin < count; begin += kTile) {
-            words_t old[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) old[i] = next[i];
-            if (begin + kTile < count) ask_rows(begin + kTile, into, ld_into);
-            quad_t acc[kOwn] = {};
-            if (adapter >= 0) {
-                const int row = order[min(begin + lane % kTile, count - 1)];
-#pragma unroll
-                for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-                    for (int half = 0; half < Inner<T>::kHalves; ++half) {
-                        const typename Op::type mine =
-                            *reinterpret_cast<const typename Op::type*>(&h[half][row][(s * kQuarters + quarter) * Op::kLane]);
-#pragma unroll
-                        for (int j = 0; j < kOwn; ++j) acc[j] = Op::mac(mine, weights[s][j], acc[j]);
-                    }
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int which = begin + quarter * 4 + i;
-                if (which >= count) continue;
-                const int row = order[which];
-                S* to = out + static_cast<size_t>(row) * ld_out + first;
-                if (whole) {
-                    float more[kOwn];
-#pragma unroll
-                    for (int j = 0; j < kOwn; ++j) more[j] = acc[j][i];
-                    *reinterpret_cast<words_t*>(to) = adapter >= 0 ? Piece<S>::sum(old[i], more) : old[i];
-                    continue;
-                }
-                const S* from = into + static_cast<size_t>(row) * ld_into + first;
-#pragma unroll
-                for (int j = 0; j < kOwn; ++j)
-                    if (first + j < end) to[j] = adapter >= 0 ? from_float<S>(to_float(from[j]) + acc[j][i]) : from[j];
-            }
-        }
-    }
-};
-
 // Four numbers of h: the parts, `apart` floats from each other, in the one order (chunks: by groups).
 __device__ __forceinline__ quad_t sum_of_parts(const float* at, size_t apart, int parts, bool chunks) {
     quad_t sum = {0.f, 0.f, 0.f, 0.f};
@@ -418,28 +339,48 @@ __device__ __forceinline__ quad_t sum_of_parts(const float* at, size_t apart, in
     return sum;
 }
 
+// A lane's numbers of its row of h (`at`), ready for the second product.
+template <typename T, int kSteps>
+__device__ __forceinline__ void ask_inner(typename Operand<T>::type (&h)[Inner<T>::kHalves][kSteps], const float* at, size_t apart, int parts,
+                                          bool chunks, float factor, int rank) {
+    typedef Operand<T> Op;
+    constexpr int kHalves = Inner<T>::kHalves;
+    const int quarter = threadIdx.x % kWave / kTile;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        const int r = (s * kQuarters + quarter) * Op::kLane;
+        typename Inner<T>::store_t both[kHalves][Op::kLane];
+#pragma unroll
+        for (int e = 0; e < Op::kLane; e += 4) {
+            quad_t sum = {0.f, 0.f, 0.f, 0.f};
+            if (r + e < rank) sum = sum_of_parts(at + r + e, apart, parts, chunks) * factor;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) Inner<T>::put(&both[0][e + i], Op::kLane, sum[i]);
+        }
+#pragma unroll
+        for (int half = 0; half < kHalves; ++half)
+#pragma unroll
+            for (int e = 0; e < Op::kLane; ++e) h[half][s][e] = both[half][e];
+    }
+}
+
 // Who of a row tile has which adapter.
 struct Order {
-    int id[kWave], order[kWave];  // the rows' adapters (-1: none, or not this workgroup's); the rows by adapter,
+    int id[kWave], order[kWave];  // the rows' adapters (-1: none); the rows by adapter,
     int group[kWave + 1], count;  // where each adapter's rows begin, and how many adapters there are
 
-    // Every `slots`-th of the adapters that the rows have; rows without one count as one more where they are to be copied.
-    __device__ __forceinline__ void sort_rows(const int* adapter, int row0, int rows, int adapters, int slots, int slot, bool copies) {
+    // (rows without an adapter count as one more where they are to be copied)
+    __device__ __forceinline__ void sort_rows(const int* adapter, int row0, int rows, int adapters, bool copies) {
         const int lane = threadIdx.x % kWave;
         if (threadIdx.x < kWave) {
             int mine = row0 + lane < rows ? adapter[row0 + lane] : -1;
             mine = mine >= 0 && mine < adapters ? mine : -1;
             u64 left = __ballot(row0 + lane < rows && (mine >= 0 || copies));
             int groups = 0, taken = 0;
-            bool own = false;
-            for (int number = 0; left; ++number) {
+            while (left) {
                 const u64 same = __ballot(mine == __builtin_amdgcn_readlane(mine, __ffsll(left) - 1)) & left;
                 left &= ~same;
-                if (number % slots != slot) continue;
-                if ((same >> lane) & 1) {
-                    own = true;
-                    order[taken + __popcll(same & ((1ull << lane) - 1))] = lane;
-                }
+                if ((same >> lane) & 1) order[taken + __popcll(same & ((1ull << lane) - 1))] = lane;
                 if (lane == 0) group[groups] = taken;
                 ++groups;
                 taken += __popcll(same);
@@ -448,13 +389,44 @@ struct Order {
                 group[groups] = taken;
                 count = groups;
             }
-            id[lane] = own ? mine : -1;
+            id[lane] = mine;
         }
         __syncthreads();
     }
 };
 
-// ... and its rows of h: the parts added in order, times the adapter's scale.
+// The same for few rows: the rows of an adapter 16 at a time, of which a workgroup has every `slots`-th sixteen.
+struct Sixteens {
+    int rows[kWave], adapter[kWave], order[kWave][kTile], count;
+
+    __device__ __forceinline__ void sort_rows(const int* adapter_of, int row0, int rows_in_all, int adapters, int slots, int slot, bool copies) {
+        const int lane = threadIdx.x % kWave;
+        if (threadIdx.x < kWave) {
+            int mine = row0 + lane < rows_in_all ? adapter_of[row0 + lane] : -1;
+            mine = mine >= 0 && mine < adapters ? mine : -1;
+            u64 left = __ballot(row0 + lane < rows_in_all && (mine >= 0 || copies));
+            int number = 0;
+            while (left) {
+                const int a = __builtin_amdgcn_readlane(mine, __ffsll(left) - 1);
+                const u64 same = __ballot(mine == a) & left;
+                left &= ~same;
+                const int in_all = __popcll(same), place = __popcll(same & ((1ull << lane) - 1)), which = number + place / kTile;
+                if ((same >> lane) & 1 && which % slots == slot) {
+                    order[which / slots][place % kTile] = lane;
+                    if (place % kTile == 0) {
+                        rows[which / slots] = min(kTile, in_all - place);
+                        adapter[which / slots] = a;
+                    }
+                }
+                number += (in_all + kTile - 1) / kTile;
+            }
+            if (lane == 0) count = number > slot ? (number - 1 - slot) / slots + 1 : 0;
+        }
+        __syncthreads();
+    }
+};
+
+// The tile's rows of h in LDS: the parts added in order, times the adapter's scale.
 template <typename T, int kSteps>
 struct Rows {
     typedef typename Inner<T>::store_t store_t;
@@ -462,11 +434,15 @@ struct Rows {
     static constexpr int kLd = kWidth + 16 / sizeof(store_t);  // (rows a little apart, so that 16 of them do not share their banks)
     store_t number[kHalves][kWave][kLd];
 
-    __device__ __forceinline__ void add_parts(const Order& tile, const float* h_part, int parts, bool chunks, const float* scale, int row0,
+    // of(i, a): the tile's row of number i below `count`, and its adapter; -1: none
+    template <typename Of>
+    __device__ __forceinline__ void add_parts(int count, Of of, const float* h_part, int parts, bool chunks, const float* scale, int row0,
                                               int rows, int inner, int from, int rank) {
         constexpr int kFours = kWidth / 4;
-        for (int item = threadIdx.x; item < kWave * kFours; item += kThreads) {
-            const int row = item / kFours, r = item % kFours * 4, a = tile.id[row];
+        for (int item = threadIdx.x; item < count * kFours; item += kThreads) {
+            const int r = item % kFours * 4;
+            int a = -1;
+            const int row = of(item / kFours, a);
             if (a < 0) continue;
             quad_t sum = {0.f, 0.f, 0.f, 0.f};
             if (r < rank)
@@ -476,6 +452,75 @@ struct Rows {
             for (int e = 0; e < 4; ++e) Inner<T>::put(&number[0][row][r + e], kWave * kLd, sum[e]);
         }
         __syncthreads();
+    }
+};
+
+// A wave's share of the second product for few rows: up to 16 rows of one adapter and a strip of columns.  h is the first operand,
+// the strip's columns the second, dealt to the instructions so that a lane's results are 16 bytes of neighbouring columns (in
+// four rows), and 16 lanes have 256 bytes of a row in one piece.
+template <typename T, typename S, int kSteps>
+struct Share {
+    typedef Operand<T> Op;
+    static constexpr int kOwn = Piece<S>::kNumbers, kStrip = kTile * kOwn, kHalves = Inner<T>::kHalves;
+    typename Op::type weights[kSteps][kOwn];
+    words_t old[4];
+    int row[4], adapter, first;  // the rows of the lane's results (-1: none) and the first of its columns
+    int mine;                    // the row that the lane brings to the product
+    bool whole;
+
+    __device__ __forceinline__ void ask(const Sixteens& tile, int which, int c0, int end, const T* up, int n, int rank, const S* into,
+                                        long ld_into, bool wide) {
+        const int lane = threadIdx.x % kWave, quarter = lane / kTile, count = tile.rows[which];
+        adapter = tile.adapter[which];
+        mine = tile.order[which][min(lane % kTile, count - 1)];
+        first = c0 + lane % kTile * kOwn;
+        whole = wide && first + kOwn <= end;
+        if (adapter >= 0) {
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j) {
+                const int c = first + j < end ? first + j : end - 1;
+                const T* from = up + (static_cast<size_t>(adapter) * n + c) * rank;
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s) weights[s][j] = up_numbers(from, (s * kQuarters + quarter) * Op::kLane, rank);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            row[i] = quarter * 4 + i < count ? tile.order[which][quarter * 4 + i] : -1;
+            if (whole && row[i] >= 0) old[i] = *reinterpret_cast<const words_t*>(into + static_cast<size_t>(row[i]) * ld_into + first);
+        }
+    }
+
+    __device__ __forceinline__ void finish(const Rows<T, kSteps>& h, int end, const S* into, long ld_into, S* out, long ld_out) {
+        const int quarter = threadIdx.x % kWave / kTile;
+        quad_t acc[kOwn] = {};
+        if (adapter >= 0) {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                for (int half = 0; half < kHalves; ++half) {
+                    const typename Op::type its =
+                        *reinterpret_cast<const typename Op::type*>(&h.number[half][mine][(s * kQuarters + quarter) * Op::kLane]);
+#pragma unroll
+                    for (int j = 0; j < kOwn; ++j) acc[j] = Op::mac(its, weights[s][j], acc[j]);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (row[i] < 0) continue;
+            S* to = out + static_cast<size_t>(row[i]) * ld_out + first;
+            if (whole) {
+                float more[kOwn];
+#pragma unroll
+                for (int j = 0; j < kOwn; ++j) more[j] = acc[j][i];
+                *reinterpret_cast<words_t*>(to) = adapter >= 0 ? Piece<S>::sum(old[i], more) : old[i];
+                continue;
+            }
+            const S* from = into + static_cast<size_t>(row[i]) * ld_into + first;
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j)
+                if (first + j < end) to[j] = adapter >= 0 ? from_float<S>(to_float(from[j]) + acc[j][i]) : from[j];
+        }
     }
 };
 
@@ -494,15 +539,17 @@ struct Columns {
     }
 };
 
-// Few rows.  grid: (row tiles, column blocks of the pieces, slots): a workgroup takes every `slots`-th of its tile's adapters, a
-// wave one of them and a strip of columns at a time.  A wave's first weights and rows of `into` are under way while the parts of h
-// are added.
+// Few rows.  grid: (row tiles, column blocks of the pieces, slots): a workgroup has every `slots`-th of its tile's sixteens, a wave
+// one of them and a strip of columns at a time.  A wave's first weights and rows of `into` are under way while the parts of h are
+// added.  (h through LDS: a wave that adds its own 16 rows' parts, without a barrier, took 20 us for 64 rows of 22,016 columns, not
+// 12.8.)  What bounds it is the way to the first result: the adapters' numbers, the parts, the weights and the barrier between
+// them; one row takes 5.4 us, 64 rows of 16 adapters 12.8 (6 MB of rows and 11 MB of weights at 1.3 TB/s).
 template <typename T, typename S, int kSteps>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kSteps == 1 ? 4 : kSteps == 2 ? 3 : 2)
 adapter_up_rows(const float* __restrict__ h_part, int parts, bool chunks, const T* __restrict__ up, const float* __restrict__ scale,
                 const int* __restrict__ adapter, const S* into, long ld_into, S* out, long ld_out, int rows, int inner, int n, int rank,
                 int adapters, Pieces pieces, int block, int slots, bool wide) {
-    __shared__ Order tile;
+    __shared__ Sixteens tile;
     __shared__ __align__(16) Rows<T, kSteps> h;
     const int wave = threadIdx.x / kWave, row0 = blockIdx.x * kWave;
     const Columns columns(pieces, blockIdx.y, block);
@@ -514,29 +561,34 @@ adapter_up_rows(const float* __restrict__ h_part, int parts, bool chunks, const 
     const int strips = (columns.end - columns.begin + kStrip - 1) / kStrip, shares = tile.count * strips;
     Share<T, S, kSteps> share;
     const auto ask = [&](int number) {
-        const int group = number / strips, from = tile.group[group];
-        share.ask(tile.order + from, tile.group[group + 1] - from, tile.id[tile.order[from]], columns.begin + number % strips * kStrip,
-                  columns.end, up, n, rank, into, ld_into, wide);
+        share.ask(tile, number / strips, columns.begin + number % strips * kStrip, columns.end, up, n, rank, into, ld_into, wide);
     };
     int number = wave;
     if (number < shares) ask(number);
-    h.add_parts(tile, h_part, parts, chunks, scale, row0, rows, inner, columns.piece * rank, rank);
+    h.add_parts(
+        tile.count * kTile,
+        [&](int i, int& a) {
+            if (i % kTile < tile.rows[i / kTile]) a = tile.adapter[i / kTile];
+            return tile.order[i / kTile][i % kTile];
+        },
+        h_part, parts, chunks, scale, row0, rows, inner, columns.piece * rank, rank);
     while (number < shares) {
-        share.finish(h.number, columns.end, into, ld_into, out, ld_out);
+        share.finish(h, columns.end, into, ld_into, out, ld_out);
         number += kWaves;
         if (number < shares) ask(number);
     }
 }
 
 // Many rows.  grid: row tiles x column blocks of the pieces, rounded up to whole turns of the XCDs: each XCD has a run of them in
-// which the row tiles of a column block follow each other, so that its L2 holds the block's weights (dealt out one by one, every
-// XCD fetched all weights: 103 us for 2,048 rows of 37,888 columns at rank 64).  A workgroup goes through its strips of columns, and in each through
-// its tile's adapters (of a prompt there is one); each of its four waves has 16 of the adapter's rows, whose h it keeps in
-// registers.  The strip's weights pass through LDS, which all four read, a strip ahead of its use.
+// which the row tiles of a column block follow each other, so that its L2 holds the block's weights.  A workgroup goes through its
+// strips of columns, and in each through its tile's adapters (of a prompt there is one); each of its four waves has 16 of the
+// adapter's rows, whose h it keeps in registers.  The strip's weights pass through LDS, which all four read, a strip ahead of
+// its use.
 //
 // The loop over whole strips has no branch around a load or store: rows that are not there have an offset behind their buffer's end,
 // which drops them.  The wait for a strip's weights then leaves the rows and stores behind them under way; with branches the
-// compiler has to wait for all of them, once a strip.
+// compiler has to wait for all of them, once a strip.  2,048 rows of 37,888 columns at rank 64, two prompts: 88 us (with the branches
+// 107) for 310 MB of rows read and written, 3.6 TB/s where a plain copy of this size reaches 5.1.
 template <typename T, typename S, int kSteps, bool kEven>  // kEven: the rank is a multiple of a lane's numbers
 __global__ void __launch_bounds__(kThreads, 4)
 adapter_up_strips(const float* __restrict__ h_part, int parts, bool chunks, const T* __restrict__ up, const float* __restrict__ scale,
@@ -562,7 +614,7 @@ adapter_up_strips(const float* __restrict__ h_part, int parts, bool chunks, cons
     if (number_of_all >= row_tiles * blocks) return;
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, quarter = lane / kTile, row0 = number_of_all % row_tiles * kWave;
     const Columns columns(pieces, number_of_all / row_tiles, block);
-    tile.sort_rows(adapter, row0, rows, adapters, 1, 0, static_cast<const void*>(into) != static_cast<const void*>(out));
+    tile.sort_rows(adapter, row0, rows, adapters, static_cast<const void*>(into) != static_cast<const void*>(out));
     if (tile.count == 0) return;
     into += static_cast<size_t>(row0) * ld_into;
     out += static_cast<size_t>(row0) * ld_out;
@@ -617,24 +669,8 @@ adapter_up_strips(const float* __restrict__ h_part, int parts, bool chunks, cons
     const auto ask_h = [&]() {  // of a tile's one adapter
         const int row = tile.order[min(wave * kTile + lane % kTile, tile.group[1] - 1)], a = tile.id[row];
         if (a < 0) return;
-        const float factor = scale[a];
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const int r = (s * kQuarters + quarter) * Op::kLane;
-            const float* at = h_part + static_cast<size_t>(row0 + row) * inner + columns.piece * rank + r;
-            store_t both[kHalves][Op::kLane];
-#pragma unroll
-            for (int e = 0; e < Op::kLane; e += 4) {
-                quad_t sum = {0.f, 0.f, 0.f, 0.f};
-                if (r + e < rank) sum = sum_of_parts(at + e, static_cast<size_t>(rows) * inner, parts, chunks) * factor;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) Inner<T>::put(&both[0][e + i], Op::kLane, sum[i]);
-            }
-#pragma unroll
-            for (int half = 0; half < kHalves; ++half)
-#pragma unroll
-                for (int e = 0; e < Op::kLane; ++e) h[half][s][e] = both[half][e];
-        }
+        ask_inner<T, kSteps>(h, h_part + static_cast<size_t>(row0 + row) * inner + columns.piece * rank, static_cast<size_t>(rows) * inner, parts,
+                             chunks, scale[a], rank);
     };
     // the strip's weights are in LDS, the next ones are asked for: what the wave's 16 rows gain
     const auto gains = [&](int number, quad_t(&acc)[kOwn]) {
@@ -666,7 +702,8 @@ adapter_up_strips(const float* __restrict__ h_part, int parts, bool chunks, cons
     ask_weights(0);
     ask_rows(0);
     if (many)
-        s_h.add_parts(tile, h_part, parts, chunks, scale, row0, rows, inner, columns.piece * rank, rank);
+        s_h.add_parts(kWave, [&](int i, int& a) { a = tile.id[i]; return i; }, h_part, parts, chunks, scale, row0, rows, inner,
+                      columns.piece * rank, rank);
     else
         ask_h();
     int number = 0;
