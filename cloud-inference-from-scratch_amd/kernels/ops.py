@@ -1609,6 +1609,44 @@ def plan_lora(rows: int, k: int, n: int, inner: int, rank: int, count: int, shar
     return chunk, parts, tile_rows, slots, block, up_slots
 
 
+@functools.lru_cache(maxsize=4096)
+def _lora_terms(x_shape, x_strides, dtype, into_shape, into_strides, out_dtype, down_shape, up_shape, out_strides, columns, units):
+    """What the shapes of :func:`lora_add`'s operands settle, checked once for each set of them (a layer calls it four times, and
+    the checks took 4 us of the host each): (rows, their distances in x, into and out, floats of the first product, the entry point's
+    numbers for 16-byte loads or None, (floats and numbers for any operands), adapters)."""
+    if len(x_shape) != 2 or len(into_shape) != 2 or len(down_shape) != 3 or len(up_shape) != 3:
+        raise ValueError(f"x {tuple(x_shape)} and into {tuple(into_shape)} must be matrices, down {tuple(down_shape)} and up "
+                         f"{tuple(up_shape)} a matrix for each adapter")
+    (rows, k), n = x_shape, into_shape[1]
+    code = _code(dtype)
+    if out_dtype is not dtype and out_dtype is not torch.float32:
+        raise ValueError(f"into must be {dtype} or float32, is {out_dtype}")
+    if into_shape[0] != rows or rows > 65535:
+        raise ValueError(f"up to 65,535 rows, as many in into as in x, not {rows} and {into_shape[0]}")
+    columns = (n,) if columns is None else columns
+    pieces = len(columns)
+    if not 1 <= pieces <= MAX_ADAPTER_PIECES or min(columns) < 1 or sum(columns) != n:
+        raise ValueError(f"columns {columns} must be 1 to {MAX_ADAPTER_PIECES} positive widths that add up to {n}")
+    count, n_up, rank = up_shape
+    if not (1 <= rank <= MAX_ADAPTER_RANK and n_up == n and down_shape == (count, pieces * rank, k) and count >= 1 and k >= 1):
+        raise ValueError(f"down {tuple(down_shape)} and up {tuple(up_shape)} do not fit rows of {k}, {n} columns in {pieces} pieces "
+                         f"and a rank of 1 to {MAX_ADAPTER_RANK}")
+    apart = []
+    for name, strides, width in (("x", x_strides, k), ("into", into_strides, n), ("out", out_strides or into_strides, n)):
+        if len(strides) != 2 or strides[1] != 1 or (rows > 1 and strides[0] < width):
+            raise ValueError(f"the rows of {name} must lie in one piece each and not overlap, its strides are {strides}")
+        apart.append(strides[0] if rows > 1 else max(strides[0], width))
+    c1 = columns[0]
+    c2 = c1 + columns[1] if pieces > 1 else n
+    numbers = (k, n, rank, count, pieces, c1, c2, c2 + columns[2] if pieces > 2 else n)
+    width = rows * pieces * rank
+    plain, size = (width, numbers + (0, 0, 0, 0, 0, 0)), 4 if code == F32 else 2
+    if rows == 0 or rank % 4 or k * size % 16 or apart[0] * size % 16:
+        return rows, *apart, 0, None, plain, count
+    plan = plan_lora(rows, k, n, pieces * rank, rank, count, 256 // size, units)
+    return rows, *apart, plan[1] * width, numbers + plan, plain, count
+
+
 def lora_add(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale: torch.Tensor, adapters: torch.Tensor,
              into: torch.Tensor, columns: Optional[tuple] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``out[t] = into[t] + scale[a] * up[a] @ (down[a] @ x[t])`` with ``a = adapters[t]``: every row's own low-rank adapter beside
@@ -1619,51 +1657,34 @@ def lora_add(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale: torch
     reads rows p R .. (p + 1) R of ``down``.  ``out`` (default: ``into`` itself) is of into's type.  x, into and out may be views
     whose rows lie apart; out is ``into`` or shares nothing with any operand.  Sums are float32, rounded once.  A row's result
     does not depend on the other rows."""
-    if x.dim() != 2 or into.dim() != 2:
-        raise ValueError(f"x {tuple(x.shape)} and into {tuple(into.shape)} must be matrices")
-    rows, k = x.shape
-    n = into.shape[1]
     dtype, out_dtype = x.dtype, into.dtype
-    code = _code(dtype)
-    if out_dtype is not dtype and out_dtype is not torch.float32:
-        raise ValueError(f"into must be {dtype} or float32, is {out_dtype}")
-    ldx = _rows_apart("x", x, rows, k, dtype)
-    ld_into = _rows_apart("into", into, rows, n, out_dtype)
-    columns = (n,) if columns is None else tuple(columns)
-    pieces = len(columns)
-    if not 1 <= pieces <= MAX_ADAPTER_PIECES or min(columns) < 1 or sum(columns) != n:
-        raise ValueError(f"columns {columns} must be 1 to {MAX_ADAPTER_PIECES} positive widths that add up to {n}")
-    _gpu("down", down, dtype, 3)
-    _gpu("up", up, dtype, 3)
-    count, n_up, rank = up.shape
-    if not (1 <= rank <= MAX_ADAPTER_RANK and n_up == n and down.shape == (count, pieces * rank, k) and count >= 1 and k >= 1):
-        raise ValueError(f"down {tuple(down.shape)} and up {tuple(up.shape)} do not fit rows of {k}, {n} columns in {pieces} pieces "
-                         f"and a rank of 1 to {MAX_ADAPTER_RANK}")
+    rows, ldx, ld_into, ld_out, floats, tiled, plain, count = _lora_terms(
+        x.shape, x.stride(), dtype, into.shape, into.stride(), out_dtype, down.shape, up.shape,
+        None if out is None or out is into else out.stride(), None if columns is None else tuple(columns), compute_units())
+    if not (down.dtype is dtype and up.dtype is dtype and down.is_contiguous() and up.is_contiguous()):
+        _gpu("down", down, dtype, 3)
+        _gpu("up", up, dtype, 3)
     _per_row("scale", scale, torch.float32, count)
     _per_row("adapters", adapters, torch.int32, rows)
-    if out is None or out is into:
-        out, ld_out = into, ld_into
-    else:
-        ld_out = _rows_apart("out", out, rows, n, out_dtype)
+    if out is None:
+        out = into
+    elif out is not into:
+        if out.dtype is not out_dtype or out.shape != into.shape:
+            raise ValueError(f"out must be {list(into.shape)} of {out_dtype}, is {tuple(out.shape)} {out.dtype}")
         if ld_out != ld_into and out.data_ptr() == into.data_ptr():
             raise ValueError("out lies where into does, with its rows at another distance")
     _on_current_gpu(x, down, up, scale, adapters, into, out)
-    if rows > 65535:
-        raise ValueError(f"up to 65,535 rows, not {rows}")
     if rows == 0:
         return out
-    size = 4 if code == F32 else 2
     x_at, down_at, up_at = x.data_ptr(), down.data_ptr(), up.data_ptr()
-    if rank % 4 == 0 and (k * size | ldx * size | x_at | down_at | up_at) % 16 == 0:
-        plan = plan_lora(rows, k, n, pieces * rank, rank, count, 256 // size, compute_units())
-    else:  # (a rank or a row that 16-byte loads do not take)
-        plan = (0, 0, 0, 0, 0, 0)
-    inner = x.new_empty((max(1, plan[1]) * rows * pieces * rank,), dtype=torch.float32)
-    c1 = columns[0]
-    c2 = c1 + columns[1] if pieces > 1 else n
+    if tiled is None or (x_at | down_at | up_at) % 16 != 0:  # (a rank, rows or a place that 16-byte loads do not take)
+        floats, terms = plain
+    else:
+        terms = tiled
+    inner = x.new_empty(floats, dtype=torch.float32)
     _run("cie_lora_add", load_library().cie_lora_add(
-        _stream(), code, _CODES[out_dtype], x_at, ldx, down_at, up_at, scale.data_ptr(), adapters.data_ptr(), into.data_ptr(), ld_into,
-        out.data_ptr(), ld_out, inner.data_ptr(), rows, k, n, rank, count, pieces, c1, c2, c2 + columns[2] if pieces > 2 else n, *plan))
+        _stream(), _CODES[dtype], _CODES[out_dtype], x_at, ldx, down_at, up_at, scale.data_ptr(), adapters.data_ptr(), into.data_ptr(),
+        ld_into, out.data_ptr(), ld_out, inner.data_ptr(), rows, *terms))
     return out
 
 
