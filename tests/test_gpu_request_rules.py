@@ -142,6 +142,14 @@ def test_temperatures_at_the_ends(ops):
         check(ops, logits.cuda(), temperature, [u] * 8, [0, 100, 0, 100, 5, 5, 1, 0], [0.9, 1.0, 0.9, 0.5, 0.5, 0.5, 0.5, 0.5])
 
 
+def test_infinite_temperatures_weigh_all_the_same(ops):
+    g = torch.Generator().manual_seed(11)
+    logits = torch.randn((6, 9001), generator=g)
+    logits[:, ::7] = -math.inf
+    check(ops, logits.cuda(), [math.inf] * 6, [0.0, 0.25, 0.5, 0.75, 0.9, LAST], [0, 0, 0, 0, 9, 0], [1.0, 1.0, 0.5, 0.5, 0.5, 1.0],
+          [1.0, 0.3, 1.0, 0.0, 1.0, 0.0])
+
+
 def test_a_weight_next_to_the_border_is_found_in_64_bits(ops):
     """Every token of 151,936 may be drawn: numbers right below and above a running share name the tokens on its two sides."""
     g = torch.Generator().manual_seed(8)
