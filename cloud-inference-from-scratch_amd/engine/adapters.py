@@ -29,7 +29,8 @@ def read_adapter(folder: str | Path) -> tuple[dict[str, torch.Tensor], float]:
         faults.append(f"peft_type {raw['peft_type']!r}")
     if raw.get("bias", "none") != "none":
         faults.append(f"bias {raw['bias']!r}")
-    faults += [f"{name} {raw[name]!r}" for name in ("use_dora", "fan_in_fan_out", "modules_to_save", "rank_pattern", "alpha_pattern")
+    faults += [f"{name} {raw[name]!r}" for name in ("use_dora", "fan_in_fan_out", "modules_to_save", "rank_pattern", "alpha_pattern",
+                                                    "lora_bias", "layer_replication", "alora_invocation_tokens")
                if raw.get(name)]
     rank, alpha = raw.get("r"), raw.get("lora_alpha")
     if not (isinstance(rank, int) and rank > 0 and isinstance(alpha, (int, float)) and math.isfinite(alpha)):
@@ -41,6 +42,9 @@ def read_adapter(folder: str | Path) -> tuple[dict[str, torch.Tensor], float]:
     for name, tensor in stored.items():
         name = name[len(_PREFIX):] if name.startswith(_PREFIX) else name
         tensors[name.replace(".lora_A.default.weight", ".lora_A.weight").replace(".lora_B.default.weight", ".lora_B.weight")] = tensor
+    others = sorted({int(t.shape[0]) for name, t in tensors.items() if name.endswith(".lora_A.weight") and t.dim() == 2} - {rank})
+    if others:
+        raise AdapterError(f"the adapter's r is {rank}, and it has matrices of rank {others}: their scale is not told")
     return tensors, alpha / (math.sqrt(rank) if raw.get("use_rslora") else rank)
 
 

@@ -166,6 +166,18 @@ def test_reading_a_folder(tmp_path):
             read_adapter(write_folder(tmp_path / "c", tensors, {**config, **change}))
 
 
+def test_a_folder_that_says_what_is_not_run(tmp_path):
+    from cie_amd.engine.adapters import read_adapter
+    from cie_amd.parts.adapters import AdapterError
+
+    tensors = adapter_tensors(TINY["A"], 4, 7)
+    config = {"peft_type": "LORA", "r": 4, "lora_alpha": 6}
+    read_adapter(write_folder(tmp_path / "a", tensors, config))
+    for change in ({"lora_bias": True}, {"layer_replication": [[0, 1], [0, 2]]}, {"alora_invocation_tokens": [5, 6]}, {"r": 8}):
+        with pytest.raises(AdapterError):
+            read_adapter(write_folder(tmp_path / "b", tensors, {**config, **change}))
+
+
 def test_names_and_slots():
     from cie_amd.engine.adapters import Adapters
     from cie_amd.parts.adapters import AdapterError, AdapterRoom
