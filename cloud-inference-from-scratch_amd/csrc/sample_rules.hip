@@ -145,6 +145,17 @@ __device__ __forceinline__ u64 partner_u64(u64 v) {
     return joined(partner<N>(static_cast<uint32_t>(v)), partner<N>(static_cast<uint32_t>(v >> 32)));
 }
 
+__device__ __forceinline__ double wave_sum_f64(double v) {  // (all lanes the same)
+    const auto with = [&](u64 other) { v += __builtin_bit_cast(double, other); };
+    with(partner_u64<1>(__builtin_bit_cast(u64, v)));
+    with(partner_u64<2>(__builtin_bit_cast(u64, v)));
+    with(partner_u64<4>(__builtin_bit_cast(u64, v)));
+    with(partner_u64<8>(__builtin_bit_cast(u64, v)));
+    with(partner_u64<16>(__builtin_bit_cast(u64, v)));
+    with(partner_u64<32>(__builtin_bit_cast(u64, v)));
+    return v;
+}
+
 // What the waves of a workgroup left in `s` (kCount of them): the sum of those in front of this one, and of all.
 template <int kCount>
 __device__ __forceinline__ void across_waves(const u64* s, u64& front, u64& total) {
@@ -398,6 +409,7 @@ rules_parts_kernel(const float* __restrict__ logits, const float* __restrict__ t
             for (int e = 0; e < 4; ++e) l[q * 4 + e] = at + e < vocab ? row[at + e] : -INFINITY;
         }
     }
+    const Rules rules(temperature, top_k, top_p, min_p, r, vocab);
     uint32_t key = 0;
     int where = 0;
 #pragma unroll
@@ -412,18 +424,13 @@ rules_parts_kernel(const float* __restrict__ logits, const float* __restrict__ t
     // the order's float (a chunk of NaN alone counts as -inf)
     const float largest = key <= kOrderOfMinusInf ? -INFINITY : logit_of(key);
     of.chunk[(static_cast<size_t>(r) * gridDim.x + part) * kPartThreads + threadIdx.x] = largest;
-#pragma unroll
-    for (int offset = kWave / 2; offset > 0; offset >>= 1) {
-        const u64 other = __shfl_xor(best, offset, kWave);
-        best = other > best ? other : best;
-    }
+    best = wave_most_u64(best);
     if (lane == 0) s_best[wave] = best;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kPartWaves; ++w) best = s_best[w] > best ? s_best[w] : best;
     PartOf::Largest* const mine = of.part + static_cast<size_t>(r) * gridDim.x + part;
     if (threadIdx.x == 0) mine->best = best;
-    const Rules rules(temperature, top_k, top_p, min_p, r, vocab);
     if (!rules.shares()) return;
     if (rules.tallied()) {  // (the launches behind this one add to them)
         for (int b = part * kPartThreads + threadIdx.x; b < kBins; b += gridDim.x * kPartThreads) of.histogram[static_cast<size_t>(r) * kBins + b] = 0;
@@ -436,8 +443,7 @@ rules_parts_kernel(const float* __restrict__ logits, const float* __restrict__ t
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum += scaled.share(l[i]);
     }
-#pragma unroll
-    for (int offset = kWave / 2; offset > 0; offset >>= 1) sum += __shfl_xor(sum, offset, kWave);
+    sum = wave_sum_f64(sum);
     if (lane == 0) s_sum[wave] = sum;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -454,54 +460,52 @@ struct Whole {
     u64 best[kBlockWaves];
     double sum[kMaxParts];  // what each part weighs
 
-    __device__ __forceinline__ u64 find_best(const PartOf::Largest* part, int parts) {
-        u64 found = 0;
-        for (int q = threadIdx.x; q < parts; q += kBlock) found = larger(found, part[q].best);
+    __device__ __forceinline__ u64 find_best(const PartOf::Largest* part, int parts, const PartOf::Largest& own) {
+        u64 found = own.best;
+        for (int q = threadIdx.x + kBlock; q < parts; q += kBlock) found = larger(found, part[q].best);
         found = wave_most_u64(found);
         if (threadIdx.x % kWave == 0) best[threadIdx.x / kWave] = found;
         __syncthreads();
         return wave_most_u64(best[threadIdx.x % kBlockWaves]);
     }
+    // (`own`: the thread's first part, asked for before anything waits)
+    static __device__ __forceinline__ PartOf::Largest first_of(const PartOf::Largest* part, int parts) {
+        return static_cast<int>(threadIdx.x) < parts ? part[threadIdx.x] : PartOf::Largest{0, 0.0};
+    }
     // (every wave the same: lanes take the parts in turn, and are added in one order)
-    __device__ __forceinline__ double find_total(const Row& row, const PartOf::Largest* part, int parts) {
+    __device__ __forceinline__ double find_total(const Row& row, const PartOf::Largest* part, int parts, const PartOf::Largest& own) {
         for (int q = threadIdx.x; q < parts; q += kBlock) {
-            const uint32_t key = static_cast<uint32_t>(part[q].best >> 32);
-            sum[q] = key > kOrderOfMinusInf ? part[q].sum * row.share(logit_of(key)) : 0.0;
+            PartOf::Largest its = own;
+            if (q >= kBlock) its = part[q];
+            const uint32_t key = static_cast<uint32_t>(its.best >> 32);
+            sum[q] = key > kOrderOfMinusInf ? its.sum * row.share(logit_of(key)) : 0.0;
         }
         __syncthreads();
         double total = 0.0;
         for (int q = threadIdx.x % kWave; q < parts; q += kWave) total += sum[q];
-        const auto with = [&](u64 other) { total += __builtin_bit_cast(double, other); };
-        with(partner_u64<1>(__builtin_bit_cast(u64, total)));
-        with(partner_u64<2>(__builtin_bit_cast(u64, total)));
-        with(partner_u64<4>(__builtin_bit_cast(u64, total)));
-        with(partner_u64<8>(__builtin_bit_cast(u64, total)));
-        with(partner_u64<16>(__builtin_bit_cast(u64, total)));
-        with(partner_u64<32>(__builtin_bit_cast(u64, total)));
-        return total;
+        return wave_sum_f64(total);
     }
 };
 
 // ---------------------------------------------------------------- rows under top-p or min-p without top-k
 // What weighs less than (1 - p) / vocab of the sum, or less than m, is not kept however the rest is shared out.
+// (In 32 bits, a little too far: the logarithm is off by some 1e-6 and 1e-7 of itself, the difference of two logits by 6e-8 of
+// itself.  In 64 bits 8 rows' tally took 9.2 us, not 8.8.)
 struct Reach {
-    float best;
-    double distance, bins;  // (and how many bins of the histogram a unit of distance has: they share the reach evenly)
+    float best, distance, bins;  // (bins: how many of the histogram's a unit of distance has; they share the reach evenly)
     __device__ __forceinline__ Reach(const Row& row, const Rules& rules, double total) {
         best = row.best;
-        const double least = rules.p < 1.0 ? fmax((1.0 - rules.p) * total / row.vocab, rules.m) : rules.m;
-        distance = -log(least) * static_cast<double>(rules.temp) * (1.0 + 1e-9) + 1e-30;  // (a little rounded up)
-        if (isnan(distance)) distance = INFINITY;  // (m = 1 at an infinite temperature: all weigh the same)
+        const float least = fmaxf(rules.p < 1.0 ? static_cast<float>((1.0 - rules.p) * total) / static_cast<float>(row.vocab) : 0.f,
+                                  static_cast<float>(rules.m));
+        distance = (2e-6f - logf(fminf(least, 1.f))) * rules.temp * 1.000002f + 1e-30f;
         bins = (kBins - 1) / distance;
     }
-    __device__ __forceinline__ bool operator()(float l) const {
-        return l > -INFINITY && (l == best || static_cast<double>(best) - static_cast<double>(l) <= distance);
-    }
+    __device__ __forceinline__ bool operator()(float l) const { return l > -INFINITY && (l == best || best - l <= distance); }
 };
 
 // The larger the nearer to the largest.
 __device__ __forceinline__ int bin_of(const Reach& reach, float l) {
-    const double at = l == reach.best ? 0.0 : (static_cast<double>(reach.best) - static_cast<double>(l)) * reach.bins;
+    const float at = l == reach.best ? 0.f : (reach.best - l) * reach.bins;
     return kBins - 1 - (at < kBins - 1 ? static_cast<int>(at) : kBins - 1);
 }
 
@@ -510,8 +514,8 @@ __device__ __forceinline__ u64 place_of(float l, int i) { return (static_cast<u6
 
 // Runs f(l, index) over the thread's chunk of a part, if its largest passes.
 template <typename F>
-__device__ __forceinline__ void walk_chunk(const Row& row, const float* chunks, int part, const Reach& reach, F f) {
-    if (!reach(chunks[part * kPartThreads + threadIdx.x])) return;
+__device__ __forceinline__ void walk_chunk(const Row& row, float largest, int part, const Reach& reach, F f) {
+    if (!reach(largest)) return;
     const int first = part * kPart + threadIdx.x * 4;
     float l[16];
     const bool lines = (reinterpret_cast<uintptr_t>(row.logits) & 15) == 0;
@@ -544,16 +548,24 @@ rules_tally_kernel(const float* __restrict__ logits, const float* __restrict__ t
     const Rules rules(temperature, top_k, top_p, min_p, r, vocab);
     if (!rules.tallied() || !(rules.p < 1.0)) return;
     const PartOf::Largest* of_parts = of.part + static_cast<size_t>(r) * parts;
+    // (what the launches before this one left is asked for at once: 8 rows' four launches 39 us, not 40)
+    const PartOf::Largest own = whole.first_of(of_parts, parts);
+    const float* chunks = of.chunk + static_cast<size_t>(r) * parts * kPartThreads + threadIdx.x;
+    float largest = chunks[blockIdx.x * kPartThreads];
     for (int b = threadIdx.x; b < kBins; b += kPartThreads) s_weight[b] = 0;
-    const uint32_t key = static_cast<uint32_t>(whole.find_best(of_parts, parts) >> 32);
+    const uint32_t key = static_cast<uint32_t>(whole.find_best(of_parts, parts, own) >> 32);
     if (key <= kOrderOfMinusInf) return;
     const Row row = {logits + static_cast<size_t>(r) * ld, vocab, logit_of(key), 1.0 / static_cast<double>(rules.temp), unit, 0.0};
-    const Reach reach(row, rules, whole.find_total(row, of_parts, parts));
-    for (int part = blockIdx.x; part < parts; part += gridDim.x)
-        walk_chunk(row, of.chunk + static_cast<size_t>(r) * parts * kPartThreads, part, reach, [&](float l, int) {
+    const Reach reach(row, rules, whole.find_total(row, of_parts, parts, own));
+    for (int part = blockIdx.x; part < parts; part += gridDim.x) {
+        const int next = part + gridDim.x < parts ? part + gridDim.x : part;
+        const float now = largest;
+        largest = chunks[next * kPartThreads];
+        walk_chunk(row, now, part, reach, [&](float l, int) {
             const u64 w = row.weight(l);
             if (w) atomicAdd(&s_weight[bin_of(reach, l)], w);
         });
+    }
     __syncthreads();
     for (int b = threadIdx.x; b < kBins; b += kPartThreads)
         if (s_weight[b]) atomicAdd(&of.histogram[static_cast<size_t>(r) * kBins + b], s_weight[b]);
@@ -572,23 +584,26 @@ rules_collect_kernel(const float* __restrict__ logits, const float* __restrict__
     const Rules rules(temperature, top_k, top_p, min_p, r, vocab);
     if (!rules.tallied()) return;
     const PartOf::Largest* of_parts = of.part + static_cast<size_t>(r) * parts;
+    const PartOf::Largest own = whole.first_of(of_parts, parts);
+    const float* chunks = of.chunk + static_cast<size_t>(r) * parts * kPartThreads + threadIdx.x;
+    float largest = chunks[blockIdx.x * kPartThreads];
     if (threadIdx.x == 0) {
         s_bin = -1;
         s_above = 0;
     }
-    const uint32_t key = static_cast<uint32_t>(whole.find_best(of_parts, parts) >> 32);
+    const uint32_t key = static_cast<uint32_t>(whole.find_best(of_parts, parts, own) >> 32);
     if (key <= kOrderOfMinusInf) return;
     const Row row = {logits + static_cast<size_t>(r) * ld, vocab, logit_of(key), 1.0 / static_cast<double>(rules.temp), unit, 0.0};
-    const double total = whole.find_total(row, of_parts, parts);
+    const double total = whole.find_total(row, of_parts, parts, own);
     const Reach reach(row, rules, total);
     if (rules.p < 1.0) {
         // the bin in which p of the weight is reached (without any, the lowest that has weight), and what lies in front of it
-        u64 own[kOwn], mine = 0;
+        u64 bins[kOwn], mine = 0;
         const u64* histogram = of.histogram + static_cast<size_t>(r) * kBins;
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) {
-            own[i] = histogram[kBins - 1 - static_cast<int>(threadIdx.x) * kOwn - i];
-            mine += own[i];
+            bins[i] = histogram[kBins - 1 - static_cast<int>(threadIdx.x) * kOwn - i];
+            mine += bins[i];
         }
         const u64 running = wave_running_u64(mine);
         if (lane == kWave - 1) s_sum[wave] = running;
@@ -600,11 +615,11 @@ rules_collect_kernel(const float* __restrict__ logits, const float* __restrict__
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) {
             // (one bin: what lies in front of it is below the limit, or nothing, and with it the limit is reached)
-            if (own[i] && (front == 0 || static_cast<double>(front) < limit) && static_cast<double>(front + own[i]) >= limit) {
+            if (bins[i] && (front == 0 || static_cast<double>(front) < limit) && static_cast<double>(front + bins[i]) >= limit) {
                 s_bin = kBins - 1 - static_cast<int>(threadIdx.x) * kOwn - i;
                 s_above = front;
             }
-            front += own[i];
+            front += bins[i];
         }
         __syncthreads();
     }
@@ -615,7 +630,10 @@ rules_collect_kernel(const float* __restrict__ logits, const float* __restrict__
         if (threadIdx.x == 0) s_count = 0;
         __syncthreads();
         u64 sum = 0;
-        walk_chunk(row, of.chunk + static_cast<size_t>(r) * parts * kPartThreads, part, reach, [&](float l, int i) {
+        const int next = part + gridDim.x < parts ? part + gridDim.x : part;
+        const float now = largest;
+        largest = chunks[next * kPartThreads];
+        walk_chunk(row, now, part, reach, [&](float l, int i) {
             const int bin = bin_of(reach, l);
             if (bin < cut_bin) return;
             const u64 w = row.weight(l);
@@ -1010,19 +1028,30 @@ __device__ int draw_of_k(const Row& row, Shared& s, const float* chunks, int chu
     return draw_from_list(row, s, n, chunk_count / kPartThreads, rules, u);
 }
 
+// What the launches before left of a tallied row, asked for before anything waits.
+struct Tallied {
+    u64 listed, above, list[kPlaces];
+    __device__ __forceinline__ void ask(Shared& s, const PartOf& of, int r, int parts) {
+        listed = of.head[2 * r];
+        above = of.head[2 * r + 1];
+#pragma unroll
+        for (int i = 0; i < kPlaces; ++i) list[i] = of.list[static_cast<size_t>(r) * kList + i * kThreads + threadIdx.x];  // (the first `listed` count)
+        for (int q = threadIdx.x; q < parts; q += kThreads) s.cut.segment[q] = of.kept[static_cast<size_t>(r) * parts + q];
+    }
+};
+
 // The draw of a row that was tallied; -2: the cut's bin holds more than its list.
-__device__ int draw_of_tally(Row& row, Shared& s, const PartOf& of, int r, int parts, const Rules& rules, double total, double u) {
-    const u64 listed = of.head[2 * r], above = of.head[2 * r + 1];
-    if (rules.p < 1.0 && listed > kList) return -2;
-    const int n = rules.p < 1.0 ? static_cast<int>(listed) : 0;
+__device__ int draw_of_tally(Row& row, Shared& s, const Tallied& tallied, int parts, const Rules& rules, double total, double u) {
+    if (rules.p < 1.0 && tallied.listed > kList) return -2;
+    const int n = rules.p < 1.0 ? static_cast<int>(tallied.listed) : 0;
     const double limit = rules.p * total * row.unit;
-    for (int q = threadIdx.x; q < parts; q += kThreads) s.cut.segment[q] = of.kept[static_cast<size_t>(r) * parts + q];
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kThreads) s.list[i] = of.list[static_cast<size_t>(r) * kList + i];
+#pragma unroll
+    for (int i = 0; i < kPlaces; ++i)
+        if (i * kThreads + static_cast<int>(threadIdx.x) < n) s.list[i * kThreads + threadIdx.x] = tallied.list[i];
     u64 cut = ~0ull;  // the last kept place
+    __syncthreads();
     if (n > 0) {
-        __syncthreads();
-        cut = cut_list(row, s, n, n, true, false, limit, rules.m, above);
+        cut = cut_list(row, s, n, n, true, false, limit, rules.m, tallied.above);
         for (int i = threadIdx.x; i < n; i += kThreads) {
             const u64 place = s.list[i];
             if (place <= cut) atomicAdd(&s.cut.segment[static_cast<uint32_t>(place) / kPart], row.weight(logit_of(~static_cast<uint32_t>(place >> 32))));
@@ -1041,7 +1070,10 @@ rules_draw_kernel(const float* __restrict__ logits, const float* __restrict__ te
     const int r = blockIdx.x;
     const PartOf::Largest* of_parts = of.part + static_cast<size_t>(r) * parts;
     const Rules rules(temperature, top_k, top_p, min_p, r, vocab);
-    const u64 best = s.whole.find_best(of_parts, parts);
+    const PartOf::Largest own = s.whole.first_of(of_parts, parts);
+    Tallied tallied;
+    if (rules.tallied()) tallied.ask(s, of, r, parts);
+    const u64 best = s.whole.find_best(of_parts, parts, own);
     const uint32_t best_key = static_cast<uint32_t>(best >> 32);
     const int best_idx = best_key > kOrderOfMinusInf ? 0x7fffffff - static_cast<int>(best & 0xffffffffu) : 0;
     if (!rules.draws() || best_key <= kOrderOfMinusInf) {
@@ -1055,10 +1087,10 @@ rules_draw_kernel(const float* __restrict__ logits, const float* __restrict__ te
     if (rules.k > 0) {
         picked = draw_of_k(row, s, of.chunk + static_cast<size_t>(r) * parts * kPartThreads, parts * kPartThreads, rules, u);
     } else {
-        const double total = s.whole.find_total(row, of_parts, parts);
+        const double total = s.whole.find_total(row, of_parts, parts, own);
         if (rules.tallied()) {
             __syncthreads();
-            picked = draw_of_tally(row, s, of, r, parts, rules, total, u);
+            picked = draw_of_tally(row, s, tallied, parts, rules, total, u);
         } else {
             __syncthreads();
             for (int q = threadIdx.x; q < parts; q += kThreads) s.cut.segment[q] = static_cast<u64>(s.whole.sum[q] * unit + 0.5);
