@@ -110,19 +110,44 @@ constexpr int kTile = 16;
 constexpr int kGroup = 4;
 constexpr int kXcds = 8;
 
-// The rows of a tile that have one adapter, first come first served: lane i learns the i-th of them.
+// Which lanes' rows have the adapter of this one's (those without an adapter belong together): a ballot for each bit of the numbers.
+// (One adapter after the other, with a ballot and a readlane for each, took 2 of 8 us where 64 rows have 16.)
+__device__ __forceinline__ u64 rows_of_same(int id, bool present, int adapters) {
+    const u64 with = __ballot(present && id >= 0), without = __ballot(present && id < 0);
+    u64 same = id >= 0 ? with : without;
+    for (int bit = 0; (adapters - 1) >> bit; ++bit) {
+        const bool set = (id >> bit) & 1;
+        const u64 ones = __ballot(set);
+        same &= set ? ones : ~ones;
+    }
+    return present ? same : 0;
+}
+__device__ __forceinline__ u64 lanes_below() { return (1ull << (threadIdx.x % kWave)) - 1; }
+// The sum of the lanes up to each one.
+template <int kControl, int kRows>
+__device__ __forceinline__ int moved(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, kControl, kRows, 0xf, false);
+}
+__device__ __forceinline__ int wave_running(int v) {
+    v += moved<0x111, 0xf>(v);
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);
+    return v + moved<0x143, 0xc>(v);
+}
+
+// The rows of a tile that have one adapter: lane i learns the i-th of them.
 struct Gathered {
     int adapter, count, row;
 };
-__device__ __forceinline__ Gathered gather(int id, u64 left) {
+__device__ __forceinline__ Gathered gather(int id, u64 mine) {
     const int lane = threadIdx.x % kWave;
     Gathered g;
-    g.adapter = __builtin_amdgcn_readlane(id, __ffsll(left) - 1);
-    const u64 mine = __ballot(id == g.adapter) & left;
+    g.adapter = __builtin_amdgcn_readlane(id, __ffsll(mine) - 1);
     g.count = __popcll(mine);
     // (the others go behind them, so that every lane is sent exactly one row)
-    const u64 below = (1ull << lane) - 1;
-    const int place = (mine >> lane) & 1 ? __popcll(mine & below) : g.count + __popcll(~mine & below);
+    const int place = (mine >> lane) & 1 ? __popcll(mine & lanes_below()) : g.count + __popcll(~mine & lanes_below());
     g.row = __builtin_amdgcn_ds_permute(place * 4, lane);
     return g;
 }
@@ -248,11 +273,12 @@ adapter_down_tiles(const T* __restrict__ x, long ldx, const T* __restrict__ down
     id = id < adapters ? id : -1;
     const int k_begin = blockIdx.x * part_k, k_end = min(k, k_begin + part_k);
     float* part = h_part + static_cast<size_t>(blockIdx.x) * rows * inner;
-    u64 left = __ballot(id >= 0);
-    for (int number = 0; left; ++number) {
-        const Gathered g = gather(id, left);
-        left &= ~__ballot(id == g.adapter);
-        if (number % slots != slot) continue;
+    const u64 same = rows_of_same(id, id >= 0, adapters);
+    const bool first = same && __ffsll(same) - 1 == lane;
+    const int running = wave_running(first), groups = __builtin_amdgcn_readlane(running, kWave - 1);
+    const int group = __shfl(running, same ? __ffsll(same) - 1 : 0, kWave) - 1;  // (in the order of their first rows)
+    for (int number = slot; number < groups; number += slots) {
+        const Gathered g = gather(id, __ballot(same && group == number));
         if (kOneTile || g.count <= kTile)
             down_rows<T, C, 1>(g, x, ldx, down, part, row0, inner, j0, k, k_begin, k_end, chunk, s_sum);
         else if constexpr (!kOneTile) {
@@ -375,19 +401,17 @@ struct Order {
         if (threadIdx.x < kWave) {
             int mine = row0 + lane < rows ? adapter[row0 + lane] : -1;
             mine = mine >= 0 && mine < adapters ? mine : -1;
-            u64 left = __ballot(row0 + lane < rows && (mine >= 0 || copies));
-            int groups = 0, taken = 0;
-            while (left) {
-                const u64 same = __ballot(mine == __builtin_amdgcn_readlane(mine, __ffsll(left) - 1)) & left;
-                left &= ~same;
-                if ((same >> lane) & 1) order[taken + __popcll(same & ((1ull << lane) - 1))] = lane;
-                if (lane == 0) group[groups] = taken;
-                ++groups;
-                taken += __popcll(same);
-            }
+            const u64 same = rows_of_same(mine, row0 + lane < rows && (mine >= 0 || copies), adapters);
+            const int place = __popcll(same & lanes_below());
+            const bool first = same && place == 0;
+            // the groups and rows in front of this lane's group, which come in the order of their first rows
+            const int own = first ? 1 << 16 | __popcll(same) : 0, running = wave_running(own);
+            const int front = __shfl(running - own, same ? __ffsll(same) - 1 : 0, kWave), all = __builtin_amdgcn_readlane(running, kWave - 1);
+            if (same) order[(front & 0xffff) + place] = lane;
+            if (first) group[front >> 16] = front & 0xffff;
             if (lane == 0) {
-                group[groups] = taken;
-                count = groups;
+                group[all >> 16] = all & 0xffff;
+                count = all >> 16;
             }
             id[lane] = mine;
         }
@@ -404,22 +428,18 @@ struct Sixteens {
         if (threadIdx.x < kWave) {
             int mine = row0 + lane < rows_in_all ? adapter_of[row0 + lane] : -1;
             mine = mine >= 0 && mine < adapters ? mine : -1;
-            u64 left = __ballot(row0 + lane < rows_in_all && (mine >= 0 || copies));
-            int number = 0;
-            while (left) {
-                const int a = __builtin_amdgcn_readlane(mine, __ffsll(left) - 1);
-                const u64 same = __ballot(mine == a) & left;
-                left &= ~same;
-                const int in_all = __popcll(same), place = __popcll(same & ((1ull << lane) - 1)), which = number + place / kTile;
-                if ((same >> lane) & 1 && which % slots == slot) {
-                    order[which / slots][place % kTile] = lane;
-                    if (place % kTile == 0) {
-                        rows[which / slots] = min(kTile, in_all - place);
-                        adapter[which / slots] = a;
-                    }
+            const u64 same = rows_of_same(mine, row0 + lane < rows_in_all && (mine >= 0 || copies), adapters);
+            const int in_all = __popcll(same), place = __popcll(same & lanes_below());
+            const int own = same && place == 0 ? (in_all + kTile - 1) / kTile : 0, running = wave_running(own);
+            const int which = __shfl(running - own, same ? __ffsll(same) - 1 : 0, kWave) + place / kTile;
+            if (same && which % slots == slot) {
+                order[which / slots][place % kTile] = lane;
+                if (place % kTile == 0) {
+                    rows[which / slots] = min(kTile, in_all - place);
+                    adapter[which / slots] = mine;
                 }
-                number += (in_all + kTile - 1) / kTile;
             }
+            const int number = __builtin_amdgcn_readlane(running, kWave - 1);
             if (lane == 0) count = number > slot ? (number - 1 - slot) / slots + 1 : 0;
         }
         __syncthreads();
