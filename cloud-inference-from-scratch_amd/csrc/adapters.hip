@@ -115,7 +115,8 @@ constexpr int kXcds = 8;
 __device__ __forceinline__ u64 rows_of_same(int id, bool present, int adapters) {
     const u64 with = __ballot(present && id >= 0), without = __ballot(present && id < 0);
     u64 same = id >= 0 ? with : without;
-    for (int bit = 0; (adapters - 1) >> bit; ++bit) {
+    const int numbers = with & (with - 1) ? adapters - 1 : 0;  // (a row alone needs none)
+    for (int bit = 0; numbers >> bit; ++bit) {
         const bool set = (id >> bit) & 1;
         const u64 ones = __ballot(set);
         same &= set ? ones : ~ones;
