@@ -10,8 +10,8 @@
 // gathered into matrix-core tiles of 16.  So no plan of who has which adapter is made on the host, a row's sums do not depend
 // on its neighbours, and a prompt (one adapter) and 64 requests (16 of them) run through the same code.
 //
-// Measured, both products, with what has to be read and written: one row of 2,048 and 2,560 columns, rank 16: 8.0 us (0.3 MB); 64
-// rows of 16 adapters, 2,048 and 22,016, rank 16: 17 us (19 MB); 24 rows of 8, 18,944 and 3,584, rank 32: 12.5 us (11.5 MB);
+// Measured, both products, with what has to be read and written: one row of 2,048 and 2,560 columns, rank 16: 8.2 us (0.3 MB); 64
+// rows of 16 adapters, 2,048 and 22,016, rank 16: 13.9 us (19 MB); 24 rows of 8, 18,944 and 3,584, rank 32: 11.1 us (11.5 MB);
 // 2,048 rows of two, 3,584 and 37,888, rank 64: 110 us (339 MB).
 #include "common.h"
 
@@ -158,7 +158,7 @@ __device__ __forceinline__ Gathered gather(int id, u64 mine) {
 // their sums through LDS, chunks are added one after the other in groups of kGroup, and the groups one after the other.  A part is
 // one chunk (few rows: as many workgroups as there are) or a group of them (many rows: fewer sums to write and read): either
 // way h is the same sum in the same order, whatever rows are beside it.  Few rows are bound by the way to their first result (one row
-// of 2,048 at rank 16 x 3: 4.0 us; 24 rows of 8 adapters, K 18,944: 6.5 us for 11 MB of weights); 2,048 rows of 3,584 at rank 64 x 2,
+// of 2,048 at rank 16 x 3: 4.0 us; 24 rows of 8 adapters, K 18,944: 6.1 us for 11 MB of weights); 2,048 rows of 3,584 at rank 64 x 2,
 // 22.6 us, by the waits of the one workgroup that each CU has (59 MB through L2: the rows for two column groups, the weights for
 // 32 row tiles; 83 TFLOP/s).  More workgroups would mean more parts to write and to add, which costs the second product more.
 template <typename T, int C, int R>
@@ -562,9 +562,9 @@ struct Columns {
 
 // Few rows.  grid: (row tiles, column blocks of the pieces, slots): a workgroup has every `slots`-th of its tile's sixteens, a wave
 // one of them and a strip of columns at a time.  A wave's first weights and rows of `into` are under way while the parts of h are
-// added.  (h through LDS: a wave that adds its own 16 rows' parts, without a barrier, took 20 us for 64 rows of 22,016 columns, not
-// 12.8.)  What bounds it is the way to the first result: the adapters' numbers, the parts, the weights and the barrier between
-// them; one row takes 5.4 us, 64 rows of 16 adapters 12.8 (6 MB of rows and 11 MB of weights at 1.3 TB/s).
+// added.  (h through LDS: a wave that adds its own 16 rows' parts, without a barrier, took 20 us for 64 rows of 22,016 columns where
+// this took 12.8.)  What bounds it is the way to the first result: the adapters' numbers, the parts, the weights and the barrier between
+// them; one row takes 5.3 us, 64 rows of 16 adapters 10.6 (6 MB of rows and 11 MB of weights at 1.6 TB/s).
 template <typename T, typename S, int kSteps>
 __global__ void __launch_bounds__(kThreads, kSteps == 1 ? 4 : kSteps == 2 ? 3 : 2)
 adapter_up_rows(const float* __restrict__ h_part, int parts, bool chunks, const T* __restrict__ up, const float* __restrict__ scale,

@@ -23,7 +23,7 @@
 //
 // One reading of the logits is what this has to cost; what few rows take beyond it are the launches' chains of small steps (find the
 // largest, add up, sort, add up, cut).  Measured, all launches: one row of 151,936 under top-k and top-p 17 us (0.6 MB; the draw
-// alone 10.6); 8 rows under top-p alone 41 us (4.9 MB; parts 7, tally 9, collect 11, draw 14); 64 rows of all kinds 65 us
+// alone 10.6); 8 rows under top-p alone 39 us (4.9 MB; parts 7, tally 9, collect 11, draw 14); 64 rows of all kinds 65 us
 // (38.9 MB; 17, 9, 12, 28); 256 rows of 152,064 under all three rules 62 us (156 MB; parts 27 at 5.7 TB/s, draw 29).  One workgroup
 // a row for all of it took 282, 400, 459 and 562 us.
 //

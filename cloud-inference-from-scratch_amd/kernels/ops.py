@@ -1592,22 +1592,22 @@ def plan_lora(rows: int, k: int, n: int, inner: int, rank: int, count: int, shar
     second product, workgroups for the adapters of its 64 rows) of :func:`lora_add`.  ``share``: the k that a workgroup takes at
     a time.  Times: both products in us.  64 rows are decoding rows of 16 adapters of rank 16 (K 2,048, 22,016 columns), 24 of
     8 of rank 32 (18,944, 3,584), 618 a batch with prompts (2,048, 2,560); 2,048 rows are two prompts (3,584, 37,888, rank 64)."""
-    # up to 16 chunks, by K alone, so that the sums are the same whatever rows come along (24 rows: 8 chunks 14.7, 15 12.8, 25 12.6)
+    # up to 16 chunks, by K alone, so that the sums are the same whatever rows come along (24 rows: 8 chunks 13.1, 15 11.1, 25 12.2)
     chunk = max(1, -(-k // (32 * share))) * 2 * share
     chunks = -(-k // chunk)
-    # a part a chunk as long as the parts are few megabytes: 24 rows 12.8 (four chunks a part: 21.4), 618 rows 14.5 (18.0); 2,048
-    # rows with four chunks a part 110 (129)
+    # a part a chunk as long as the parts are few megabytes: 24 rows 11.1 (four chunks a part: 20.6), 618 rows 14.0 (17.7); 2,048
+    # rows with four chunks a part 111 (129)
     parts = chunks if rows * inner * chunks <= 1 << 20 else -(-chunks // 4)
-    # 64 rows read the weights once, 16 make more workgroups: 2,048 rows 110 (16 rows: 115), 618 rows 16.0 (14.5)
+    # 64 rows read the weights once, 16 make more workgroups: 2,048 rows 111 (16 rows: 118), 618 rows 15.5 (14.0)
     tile_rows = 64 if -(-rows // 64) * -(-inner // 64) * parts >= units else 16
-    # decoding rows have an adapter each, a prompt's tile has one or two: 64 rows 17.2 (2 workgroups: 25.5), 618 rows 14.5 (16: 17.1)
+    # decoding rows have an adapter each, a prompt's tile has one or two: 64 rows 13.9 (2 workgroups: 19.3), 618 rows 14.0 (16: 17.0)
     slots = min(count, rows, 16 if rows <= 128 else 2)
-    # the second product's form for many rows where it fills the GPU: 2,048 rows 110 (the other form: 218), 618 rows 19.4 (14.5); it
-    # takes one turn of four workgroups a CU (a strip each: 155)
+    # the second product's form for many rows where it fills the GPU: 2,048 rows 111 (the other form: 218), 618 rows 19.2 (14.0); it
+    # takes one turn of four workgroups a CU (a strip each: 158)
     tiles, strips = -(-rows // 64), -(-n // 128)
     many = tiles * strips >= 4 * units and rank <= 64
     block = 128 * (-(-strips * tiles // (4 * units)) if many else 1)
-    # the adapters of 64 rows: 24 rows 12.8 (4 workgroups: 15.5), where 8 no longer run at once 64 rows 17.2 (8: 20.4)
+    # the adapters of 64 rows: 24 rows 11.1 (4 workgroups: 13.9), where 8 no longer run at once 64 rows 13.9 (8: 14.9)
     up_slots = 0 if many else min(rows, 8 if 8 * tiles * strips <= 4 * units else 4)
     return chunk, parts, tile_rows, slots, block, up_slots
 
