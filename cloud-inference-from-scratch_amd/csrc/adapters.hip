@@ -188,7 +188,8 @@ __device__ __forceinline__ void down_rows(const Gathered& g, const T* __restrict
 #pragma unroll
         for (int c = 0; c < C; ++c) acc[i][c] = quad_t{0.f, 0.f, 0.f, 0.f};
     }
-    // a round is U steps of every wave (U of 1: 2,048 rows 24 us, not 22); the next round is under way while one is multiplied, also across the end of a chunk
+    // a round is U steps of every wave (U of 1: 2,048 rows 24 us, not 22); the next round is under way while one is multiplied, also
+    // across the end of a chunk
     constexpr int U = 2, kRound = kStep * kWaves * U;
     const int rounds = (k_end - k_begin + kRound - 1) / kRound, rounds_of_chunk = chunk / kRound;
     typename Op::type a[U][R], b[U][C];
@@ -812,7 +813,8 @@ int run_tiles(hipStream_t s, const void* x_, long ldx, const void* down_, const 
     if (plan.up_slots > 0) {
 #define CIE_UP(STEPS)                                                                                                              \
     adapter_up_rows<T, S, STEPS><<<dim3(row_tiles, blocks, plan.up_slots), kThreads, 0, s>>>(                                          \
-        h, plan.parts, plan.chunks(k), up, scale, adapter, into, ld_into, out, ld_out, rows, inner, n, rank, adapters, pieces, plan.block, plan.up_slots, wide)
+        h, plan.parts, plan.chunks(k), up, scale, adapter, into, ld_into, out, ld_out, rows, inner, n, rank, adapters, pieces, plan.block,  \
+        plan.up_slots, wide)
         if (rank <= kStep)
             CIE_UP(1);
         else if (rank <= 2 * kStep)
@@ -859,7 +861,7 @@ CIE_API int cie_lora_add(void* stream, int dtype, int out_dtype, const void* x, 
                          const float* scale, const int* adapter, const void* into, long ld_into, void* out, long ld_out, float* h,
                          int rows, int k, int n, int rank, int adapters, int piece_count, int c1, int c2, int c3, int chunk,
                          int parts, int tile_rows, int slots, int block, int up_slots) {
-    if (rows < 0 || rows > 65535 || k <= 0 || n <= 0 || rank <= 0 || rank > 128 || adapters <= 0 || piece_count < 1 ||
+    if (rows < 0 || rows > 65535 || k <= 0 || k > (1 << 28) || n <= 0 || n > (1 << 28) || rank <= 0 || rank > 128 || adapters <= 0 || piece_count < 1 ||
         piece_count > kMaxPieces || ldx < k || ld_into < n || ld_out < n || !x || !down || !up || !scale || !adapter || !into || !out || !h)
         return CIE_BAD_ARGUMENT;
     if (rows == 0) return CIE_OK;
@@ -874,9 +876,10 @@ CIE_API int cie_lora_add(void* stream, int dtype, int out_dtype, const void* x, 
                            reinterpret_cast<uintptr_t>(down) % 16 == 0 && reinterpret_cast<uintptr_t>(up) % 16 == 0 &&
                            reinterpret_cast<uintptr_t>(h) % 16 == 0;
         const int share = 256 / size;  // (the k that a workgroup's four waves take at a time)
-        if (!lines || rank % 4 || chunk < 2 * share || chunk % (2 * share) || (parts != (k + chunk - 1) / chunk && parts != (k + kGroup * chunk - 1) / (kGroup * chunk)) || tile_rows < 16 ||
-            tile_rows > kWave || tile_rows % kTile || slots < 1 || slots > kWave || block < kWave || block % kWave || up_slots < 0 ||
-            up_slots > kWave || (up_slots == 0 && rank > 64))
+        if (!lines || rank % 4 || chunk < 2 * share || chunk % (2 * share) ||
+            (!plan.chunks(k) && parts != (k + kGroup * chunk - 1) / (kGroup * chunk)) || tile_rows < 16 || tile_rows > kWave ||
+            tile_rows % kTile || slots < 1 || slots > kWave || block < kWave || block % kWave || up_slots < 0 || up_slots > kWave ||
+            (up_slots == 0 && rank > 64))
             return CIE_BAD_ARGUMENT;
     }
     hipStream_t s = static_cast<hipStream_t>(stream);

@@ -1626,6 +1626,8 @@ def _lora_terms(x_shape, x_strides, dtype, into_shape, into_strides, out_dtype, 
         raise ValueError(f"into must be {dtype} or float32, is {out_dtype}")
     if into_shape[0] != rows or rows > 65535:
         raise ValueError(f"up to 65,535 rows, as many in into as in x, not {rows} and {into_shape[0]}")
+    if max(k, n) > 1 << 28:
+        raise ValueError(f"rows of up to {1 << 28} numbers, not {k} and {n}")
     columns = (n,) if columns is None else columns
     pieces = len(columns)
     if not 1 <= pieces <= MAX_ADAPTER_PIECES or min(columns) < 1 or sum(columns) != n:

@@ -98,6 +98,16 @@ def test_odd_columns(ops, dtype, stream, columns):
 
 
 @pytest.mark.parametrize("dtype,stream", KINDS)
+def test_numbers_of_many_adapters(ops, dtype, stream):
+    """Numbers that differ in a single bit, low or high, beside rows without any."""
+    bits = [1 << b for b in range(10)]
+    adapters = [0, *bits, -1, 1023, *[1023 - b for b in bits], 0, 512, 513, *range(300, 340), -1, 1000, 1000, 512]
+    for rows in (len(adapters), 16, 3):
+        check(ops, site(rows, 64, (40,), 4, 1024, getattr(torch, dtype), stream, seed=rows, adapters=adapters[-rows:]))
+    check(ops, site(4000, 64, (2048, 2048), 4, 1024, getattr(torch, dtype), stream, seed=9, adapters=(adapters * 60)[:4000]))
+
+
+@pytest.mark.parametrize("dtype,stream", KINDS)
 def test_who_has_which_adapter(ops, dtype, stream):
     """None at all, one for all, every row another one, runs that end inside a tile, numbers that name no adapter."""
     for seed, adapters in enumerate([

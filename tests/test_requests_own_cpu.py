@@ -245,3 +245,16 @@ def test_log_probabilities_reach_the_request():
     assert asks.output == [100, 101, 102] and asks.logprobs == [-25.0, -25.25, -25.5]
     assert silent.output == [100, 101, 102] and silent.logprobs == []
     assert all(type(token) is int for token in asks.output)
+
+
+def test_rows_too_long_for_the_kernels_indexes():
+    from cie_amd.kernels import ops
+
+    def terms(k, n):
+        return ops._lora_terms(torch.Size((1, k)), (k, 1), torch.bfloat16, torch.Size((1, n)), (n, 1), torch.bfloat16, torch.Size((1, 8, k)),
+                               torch.Size((1, n, 8)), None, None, 256)
+
+    assert terms(1 << 28, 64)[0] == terms(64, 1 << 28)[0] == 1
+    for k, n in (((1 << 28) + 8, 64), (64, (1 << 28) + 8)):
+        with pytest.raises(ValueError):
+            terms(k, n)
