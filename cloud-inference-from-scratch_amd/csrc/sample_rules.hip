@@ -799,6 +799,7 @@ struct Shared {
     };
     u64 sum[kWaves];
     int count, hit_count;
+    int picked;  // what one wave draws alone (not in `count`, which the other waves may still have to read then)
 };
 
 // The smallest of the threads' first choices (kNone: none), the largest of their second ones (-1) if there is none.
@@ -941,10 +942,10 @@ __device__ int draw_from_list(const Row& row, Shared& s, int n, int parts, const
             const u64 kept = wave_sort(weight ? place << 32 | place >> 32 : ~0ull);  // by index
             weight = kept != ~0ull ? row.weight(logit_of(~static_cast<uint32_t>(kept))) : 0;
             const int which = pick_lane(weight, u);
-            if (lane == max(0, which)) s.count = which < 0 ? -1 : static_cast<int>(kept >> 32);
+            if (lane == max(0, which)) s.picked = which < 0 ? -1 : static_cast<int>(kept >> 32);
         }
         __syncthreads();
-        return s.count;
+        return s.picked;
     }
     const u64 cut = cut_list(row, s, n, rules.k, rules.p < 1.0, true, rules.p, rules.m, 0);
     // where the kept ones lie: the parts' sums

@@ -303,3 +303,25 @@ def test_refusals(ops):
         given.update(change)
         with pytest.raises(ValueError):
             ops.token_logprobs(**given)
+
+
+def test_short_lists_of_many_rows_at_once(ops):
+    """Rows that one wave finishes alone, several workgroups a unit, with work of another stream beside them: the number that the
+    wave draws must not be taken for the list's length by a wave that comes late."""
+    g = torch.Generator().manual_seed(41)
+    rows, vocab = 1500, 9001
+    logits = torch.randn((rows, vocab), generator=g) * 3
+    uniform, k = torch.rand(rows, generator=g).tolist(), [1 + r % 50 for r in range(rows)]
+    want = expected(logits, [1.0] * rows, uniform, k)
+    assert sum(64 < token <= 4096 for token in want) > 300 and sum(token > 4096 for token in want) > 300
+    on = logits.cuda(), torch.ones(rows).cuda(), torch.tensor(uniform).cuda(), torch.tensor(k, dtype=torch.int32).cuda()
+    beside = torch.randn((4096, 4096), generator=g).cuda()
+    torch.cuda.synchronize()
+    side, got = torch.cuda.Stream(), []
+    for _ in range(6):
+        with torch.cuda.stream(side):
+            beside = torch.sin(beside)
+        got.append(ops.sample(*on[:3], top_k=on[3]))
+    torch.cuda.synchronize()
+    for tokens in got:
+        assert tokens.tolist() == want
