@@ -881,6 +881,9 @@ CIE_API int cie_lora_add(void* stream, int dtype, int out_dtype, const void* x, 
             tile_rows % kTile || slots < 1 || slots > kWave || block < kWave || block % kWave || up_slots < 0 || up_slots > kWave ||
             (up_slots == 0 && rank > 64))
             return CIE_BAD_ARGUMENT;
+        long blocks = 0;
+        for (int p = 0; p < piece_count; ++p) blocks += (pieces.begin[p + 1] - pieces.begin[p] + block - 1) / block;
+        if (up_slots > 0 && blocks > 65535) return CIE_BAD_ARGUMENT;  // (a grid's second dimension)
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
 #define CIE_RUN(T, S)                                                                                                              \

@@ -1606,7 +1606,8 @@ def plan_lora(rows: int, k: int, n: int, inner: int, rank: int, count: int, shar
     # takes one turn of four workgroups a CU (a strip each: 158)
     tiles, strips = -(-rows // 64), -(-n // 128)
     many = tiles * strips >= 4 * units and rank <= 64
-    block = 128 * (-(-strips * tiles // (4 * units)) if many else 1)
+    # (the other form's column blocks are a grid's second dimension, which ends at 65,535: one more for each piece that a block ends with)
+    block = 128 * -(-strips * tiles // (4 * units) if many else -strips // (65535 - MAX_ADAPTER_PIECES))
     # the adapters of 64 rows: 24 rows 11.1 (4 workgroups: 13.9), where 8 no longer run at once 64 rows 13.9 (8: 14.9)
     up_slots = 0 if many else min(rows, 8 if 8 * tiles * strips <= 4 * units else 4)
     return chunk, parts, tile_rows, slots, block, up_slots

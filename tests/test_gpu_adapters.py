@@ -220,3 +220,28 @@ def test_refusals(ops):
     wide = {name: value.cuda() if torch.is_tensor(value) else value for name, value in site(4, 64, (32,), 8, 2, torch.float32).items()}
     with pytest.raises(ValueError):
         ops.lora_add(**dict(wide, into=wide["into"].bfloat16()))
+
+
+def test_more_columns_than_a_grids_second_dimension_has_blocks(ops):
+    """Few rows of a rank that the form for many does not take; the widths end inside a block."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    columns = (8388480, 333, 70001)
+    n, rank, k = sum(columns), 72, 8
+    x = torch.randn((2, k), generator=g, device="cuda").bfloat16()
+    down = torch.randn((2, 3 * rank, k), generator=g, device="cuda").bfloat16()
+    up = torch.randn((2, n, rank), generator=g, device="cuda").bfloat16()
+    scale, adapters = torch.tensor([0.5, 1.5], device="cuda"), torch.tensor([1, 0], dtype=torch.int32, device="cuda")
+    into = torch.randn((2, n), generator=g, device="cuda")
+    got = ops.lora_add(x, down, up, scale, adapters, into, columns=columns, out=torch.empty_like(into))
+    begin = 0
+    for piece, width in enumerate(columns):
+        for first in range(begin, begin + width, 1 << 20):
+            part = slice(first, min(first + (1 << 20), begin + width))
+            for row, a in enumerate((1, 0)):
+                inner = down[a, piece * rank: (piece + 1) * rank].double() * x[row].double()
+                factor = up[a, part].double()
+                want = into[row, part].double() + scale[a].double() * (factor @ inner.sum(1))
+                size = scale[a].double() * (factor.abs() @ inner.abs().sum(1))
+                bound = size * ((k + rank + 8) * 2.0 ** -24 + 2.0 ** -17) + want.abs() * 2.0 ** -22  # (as definition() has it)
+                assert ((got[row, part].double() - want).abs() <= bound).all(), (piece, first, row)
+        begin += width

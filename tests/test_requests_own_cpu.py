@@ -258,3 +258,20 @@ def test_rows_too_long_for_the_kernels_indexes():
     for k, n in (((1 << 28) + 8, 64), (64, (1 << 28) + 8)):
         with pytest.raises(ValueError):
             terms(k, n)
+
+
+def test_column_blocks_stay_in_a_grids_second_dimension():
+    """The form for few rows has its column blocks there: for the widest rows, any rank and pieces of any width."""
+    from cie_amd.kernels import ops
+
+    forms = set()
+    for n in (1, 128, 2560, 37888, 8388480, 8388609, 9000000, 1 << 28):
+        for rows in (1, 64, 618, 65535):
+            for rank in (1, 8, 64, 72, 128):
+                *_, block, up_slots = ops.plan_lora(rows, 64, n, 4 * rank, rank, 3, 128, 256)
+                assert block % 128 == 0
+                if up_slots:
+                    widths = [n] if n < 4 else [1, 1, n // 2, n - n // 2 - 2]
+                    assert sum(-(-width // block) for width in widths) <= 65535, (n, rows, rank)
+                    forms.add(block)
+    assert len(forms) > 2 and ops.plan_lora(64, 2048, 22016, 32, 16, 16, 128, 256)[4] == 128  # (as it is for a model's widths)
