@@ -4,7 +4,7 @@
 // projections that read the same rows (q, k and v; gate and up): `down` [A, P R, K] has R rows for each, the columns of `out`
 // fall into P pieces, and p(c) is the piece of column c.
 //
-// The sums are float32, the result is rounded once.  Two launches: `down` (K long, few columns; K cut into parts whose float32 sums
+// The sums are float32, the result is rounded once (h on its way onto rows of bfloat16 keeps 16 bits).  Two launches: `down` (K long, few columns; K cut into parts whose float32 sums
 // lie side by side, so that few rows still fill the GPU) and `up` (R long, many columns; it adds the parts in order).  Rows are
 // taken in tiles of consecutive ones; what a tile does is done once for each adapter that its rows have, on these rows alone,
 // gathered into matrix-core tiles of 16.  So no plan of who has which adapter is made on the host, a row's sums do not depend
@@ -292,25 +292,28 @@ adapter_down_tiles(const T* __restrict__ x, long ldx, const T* __restrict__ down
     }
 }
 
-// The rows of h on their way into the second product.  In bfloat16 a number is two: its rounding and the rounding of what that
-// left out, 16 bits together (2^-17 of the number), so that a float32 stream does not lose the adapter's low bits; the
-// product runs twice, which its 16 to 128 long sums never notice beside the rows they are added to.
-template <typename T>
+// The rows of h on their way into the second product, whose result is of type S.  In bfloat16 a number is the sum of several: its
+// rounding, the rounding of what that left out, and so on, 8 bits each, and the product runs once for each.  A float32 stream has all
+// three that a float32 number holds; rows of bfloat16, which keep 8 bits of the sum, two (2^-17 of the number).
+template <typename T, typename S>
 struct Inner;
-template <>
-struct Inner<bf16_t> {
-    static constexpr int kHalves = 2;
+template <typename S>
+struct Inner<bf16_t, S> {
+    static constexpr int kTerms = sizeof(S) == 4 ? 3 : 2;
     typedef __bf16 store_t;
     static __device__ __forceinline__ void put(store_t* at, int apart, float v) {
-        const __bf16 high = static_cast<__bf16>(v);
-        const float kept = static_cast<float>(high);
-        at[0] = high;
-        at[apart] = static_cast<__bf16>(fabsf(kept) < INFINITY ? v - kept : 0.f);
+#pragma unroll
+        for (int i = 0; i < kTerms; ++i) {
+            const __bf16 term = static_cast<__bf16>(v);
+            const float kept = static_cast<float>(term);
+            at[i * apart] = term;
+            v = fabsf(kept) < INFINITY ? v - kept : 0.f;  // (exact)
+        }
     }
 };
 template <>
-struct Inner<float> {
-    static constexpr int kHalves = 1;
+struct Inner<float, float> {
+    static constexpr int kTerms = 1;
     typedef float store_t;
     static __device__ __forceinline__ void put(store_t* at, int, float v) { at[0] = v; }
 };
@@ -368,27 +371,27 @@ __device__ __forceinline__ quad_t sum_of_parts(const float* at, size_t apart, in
 }
 
 // A lane's numbers of its row of h (`at`), ready for the second product.
-template <typename T, int kSteps>
-__device__ __forceinline__ void ask_inner(typename Operand<T>::type (&h)[Inner<T>::kHalves][kSteps], const float* at, size_t apart, int parts,
-                                          bool chunks, float factor, int rank) {
+template <typename T, typename S, int kSteps, int kTerms>
+__device__ __forceinline__ void ask_inner(typename Operand<T>::type (&h)[kTerms][kSteps], const float* at, size_t apart, int parts, bool chunks,
+                                          float factor, int rank) {
     typedef Operand<T> Op;
-    constexpr int kHalves = Inner<T>::kHalves;
+    static_assert(kTerms == Inner<T, S>::kTerms, "room for all terms");
     const int quarter = threadIdx.x % kWave / kTile;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
         const int r = (s * kQuarters + quarter) * Op::kLane;
-        typename Inner<T>::store_t both[kHalves][Op::kLane];
+        typename Inner<T, S>::store_t terms[kTerms][Op::kLane];
 #pragma unroll
         for (int e = 0; e < Op::kLane; e += 4) {
             quad_t sum = {0.f, 0.f, 0.f, 0.f};
             if (r + e < rank) sum = sum_of_parts(at + r + e, apart, parts, chunks) * factor;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) Inner<T>::put(&both[0][e + i], Op::kLane, sum[i]);
+            for (int i = 0; i < 4; ++i) Inner<T, S>::put(&terms[0][e + i], Op::kLane, sum[i]);
         }
 #pragma unroll
-        for (int half = 0; half < kHalves; ++half)
+        for (int term = 0; term < kTerms; ++term)
 #pragma unroll
-            for (int e = 0; e < Op::kLane; ++e) h[half][s][e] = both[half][e];
+            for (int e = 0; e < Op::kLane; ++e) h[term][s][e] = terms[term][e];
     }
 }
 
@@ -449,12 +452,12 @@ struct Sixteens {
 };
 
 // The tile's rows of h in LDS: the parts added in order, times the adapter's scale.
-template <typename T, int kSteps>
+template <typename T, typename S, int kSteps>
 struct Rows {
-    typedef typename Inner<T>::store_t store_t;
-    static constexpr int kWidth = kSteps * Operand<T>::kLane * kQuarters, kHalves = Inner<T>::kHalves;
+    typedef typename Inner<T, S>::store_t store_t;
+    static constexpr int kWidth = kSteps * Operand<T>::kLane * kQuarters, kTerms = Inner<T, S>::kTerms;
     static constexpr int kLd = kWidth + 16 / sizeof(store_t);  // (rows a little apart, so that 16 of them do not share their banks)
-    store_t number[kHalves][kWave][kLd];
+    store_t number[kTerms][kWave][kLd];
 
     // of(i, a): the tile's row of number i below `count`, and its adapter; -1: none
     template <typename Of>
@@ -471,7 +474,7 @@ struct Rows {
                 sum = sum_of_parts(h_part + static_cast<size_t>(row0 + row) * inner + from + r, static_cast<size_t>(rows) * inner, parts, chunks) *
                       scale[a];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) Inner<T>::put(&number[0][row][r + e], kWave * kLd, sum[e]);
+            for (int e = 0; e < 4; ++e) Inner<T, S>::put(&number[0][row][r + e], kWave * kLd, sum[e]);
         }
         __syncthreads();
     }
@@ -483,7 +486,7 @@ struct Rows {
 template <typename T, typename S, int kSteps>
 struct Share {
     typedef Operand<T> Op;
-    static constexpr int kOwn = Piece<S>::kNumbers, kStrip = kTile * kOwn, kHalves = Inner<T>::kHalves;
+    static constexpr int kOwn = Piece<S>::kNumbers, kStrip = kTile * kOwn, kTerms = Inner<T, S>::kTerms;
     typename Op::type weights[kSteps][kOwn];
     words_t old[4];
     int row[4], adapter, first;  // the rows of the lane's results (-1: none) and the first of its columns
@@ -513,16 +516,16 @@ struct Share {
         }
     }
 
-    __device__ __forceinline__ void finish(const Rows<T, kSteps>& h, int end, const S* into, long ld_into, S* out, long ld_out) {
+    __device__ __forceinline__ void finish(const Rows<T, S, kSteps>& h, int end, const S* into, long ld_into, S* out, long ld_out) {
         const int quarter = threadIdx.x % kWave / kTile;
         quad_t acc[kOwn] = {};
         if (adapter >= 0) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-                for (int half = 0; half < kHalves; ++half) {
+                for (int term = 0; term < kTerms; ++term) {
                     const typename Op::type its =
-                        *reinterpret_cast<const typename Op::type*>(&h.number[half][mine][(s * kQuarters + quarter) * Op::kLane]);
+                        *reinterpret_cast<const typename Op::type*>(&h.number[term][mine][(s * kQuarters + quarter) * Op::kLane]);
 #pragma unroll
                     for (int j = 0; j < kOwn; ++j) acc[j] = Op::mac(its, weights[s][j], acc[j]);
                 }
@@ -572,7 +575,7 @@ adapter_up_rows(const float* __restrict__ h_part, int parts, bool chunks, const 
                 const int* __restrict__ adapter, const S* into, long ld_into, S* out, long ld_out, int rows, int inner, int n, int rank,
                 int adapters, Pieces pieces, int block, int slots, bool wide) {
     __shared__ Sixteens tile;
-    __shared__ __align__(16) Rows<T, kSteps> h;
+    __shared__ __align__(16) Rows<T, S, kSteps> h;
     const int wave = threadIdx.x / kWave, row0 = blockIdx.x * kWave;
     const Columns columns(pieces, blockIdx.y, block);
     tile.sort_rows(adapter, row0, rows, adapters, slots, blockIdx.z, static_cast<const void*>(into) != static_cast<const void*>(out));
@@ -617,10 +620,10 @@ adapter_up_strips(const float* __restrict__ h_part, int parts, bool chunks, cons
                   const int* __restrict__ adapter, const S* into, long ld_into, S* out, long ld_out, int rows, int inner, int n, int rank,
                   int adapters, Pieces pieces, int block, int row_tiles, int blocks, bool wide) {
     typedef Operand<T> Op;
-    typedef typename Inner<T>::store_t store_t;
+    typedef typename Inner<T, S>::store_t store_t;
     constexpr int kOwn = Piece<S>::kNumbers, kStrip = kTile * kOwn, kLoads = kSteps * kQuarters, kMine = kStrip * kLoads / kThreads;
-    typedef Rows<T, kSteps> RowsT;
-    constexpr int kLd = RowsT::kLd, kHalves = RowsT::kHalves;
+    typedef Rows<T, S, kSteps> RowsT;
+    constexpr int kLd = RowsT::kLd, kTerms = RowsT::kTerms;
     static_assert(kStrip * kLoads % kThreads == 0, "every thread stages as many pieces");
     __shared__ Order tile;
     // Two buffers of weights in turn.  A tile of several adapters has them one after the other in the first, with a barrier more,
@@ -651,7 +654,7 @@ adapter_up_strips(const float* __restrict__ h_part, int parts, bool chunks, cons
     const int whole = wide ? (columns.end - columns.begin) / kStrip * groups : 0;
     const bool many = groups > 1;
 
-    typename Op::type staged[kMine], h[kHalves][kSteps];
+    typename Op::type staged[kMine], h[kTerms][kSteps];
     words_t old[4];
     const auto ask_weights = [&](int number) {
         const int a = max(0, tile.id[tile.order[tile.group[number % groups]]]);  // (rows without an adapter: not used)
@@ -691,8 +694,8 @@ adapter_up_strips(const float* __restrict__ h_part, int parts, bool chunks, cons
     const auto ask_h = [&]() {  // of a tile's one adapter
         const int row = tile.order[min(wave * kTile + lane % kTile, tile.group[1] - 1)], a = tile.id[row];
         if (a < 0) return;
-        ask_inner<T, kSteps>(h, h_part + static_cast<size_t>(row0 + row) * inner + columns.piece * rank, static_cast<size_t>(rows) * inner, parts,
-                             chunks, scale[a], rank);
+        ask_inner<T, S, kSteps>(h, h_part + static_cast<size_t>(row0 + row) * inner + columns.piece * rank, static_cast<size_t>(rows) * inner,
+                                parts, chunks, scale[a], rank);
     };
     // the strip's weights are in LDS, the next ones are asked for: what the wave's 16 rows gain
     const auto gains = [&](int number, quad_t(&acc)[kOwn]) {
@@ -706,10 +709,10 @@ adapter_up_strips(const float* __restrict__ h_part, int parts, bool chunks, cons
         if (many) {
             const int row = tile.order[from + min(wave * kTile + lane % kTile, count - 1)];
 #pragma unroll
-            for (int half = 0; half < kHalves; ++half)
+            for (int term = 0; term < kTerms; ++term)
 #pragma unroll
                 for (int s = 0; s < kSteps; ++s)
-                    h[half][s] = *reinterpret_cast<const typename Op::type*>(&s_h.number[half][row][(s * kQuarters + quarter) * Op::kLane]);
+                    h[term][s] = *reinterpret_cast<const typename Op::type*>(&s_h.number[term][row][(s * kQuarters + quarter) * Op::kLane]);
         }
 #pragma unroll
         for (int s = 0; s < kSteps; ++s)
@@ -718,7 +721,7 @@ adapter_up_strips(const float* __restrict__ h_part, int parts, bool chunks, cons
                 const typename Op::type weights =
                     *reinterpret_cast<const typename Op::type*>(&s_w[buffer].number[j * kTile + lane % kTile][(s * kQuarters + quarter) * Op::kLane]);
 #pragma unroll
-                for (int half = 0; half < kHalves; ++half) acc[j] = Op::mac(h[half][s], weights, acc[j]);
+                for (int term = 0; term < kTerms; ++term) acc[j] = Op::mac(h[term][s], weights, acc[j]);
             }
     };
     ask_weights(0);

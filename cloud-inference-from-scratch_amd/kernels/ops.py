@@ -1661,8 +1661,8 @@ def lora_add(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale: torch
     x [T, K]; down [A, P * R, K]; up [A, N, R]; scale float32 [A]; adapters int32 [T]; into [T, N] in x's type or float32 (the
     residual stream).  ``columns``: the widths of the P projections that are stacked in the N columns (default: one); projection p
     reads rows p R .. (p + 1) R of ``down``.  ``out`` (default: ``into`` itself) is of into's type.  x, into and out may be views
-    whose rows lie apart; out is ``into`` or shares nothing with any operand.  Sums are float32, rounded once.  A row's result
-    does not depend on the other rows."""
+    whose rows lie apart; out is ``into`` or shares nothing with any operand.  Sums are float32, rounded once; onto rows of
+    bfloat16 the inner products enter the second sum with 16 bits.  A row's result does not depend on the other rows."""
     dtype, out_dtype = x.dtype, into.dtype
     rows, ldx, ld_into, ld_out, floats, tiled, plain, count = _lora_terms(
         x.shape, x.stride(), dtype, into.shape, into.stride(), out_dtype, down.shape, up.shape,

@@ -245,3 +245,29 @@ def test_more_columns_than_a_grids_second_dimension_has_blocks(ops):
                 bound = size * ((k + rank + 8) * 2.0 ** -24 + 2.0 ** -17) + want.abs() * 2.0 ** -22  # (as definition() has it)
                 assert ((got[row, part].double() - want).abs() <= bound).all(), (piece, first, row)
         begin += width
+
+
+@pytest.mark.parametrize("rank", [3, 4, 8, 16, 24, 32, 40, 64, 72, 128])
+@pytest.mark.parametrize("rows,columns", [(1, 48), (37, 200), (2048, 4300)])
+def test_the_streams_sums_keep_all_bits_of_32(ops, rows, columns, rank):
+    """bfloat16 operands whose inner products are whole numbers of 24 bits times a power of two (three digits of 8 bits), each
+    times a single 1 of `up`, into a float32 stream of zeros: every step is exact in 32 bits, so the result has to be equal."""
+    g = torch.Generator().manual_seed(rows + rank)
+    digits = torch.randint(128, 256, (2, rank, 3), generator=g) * (2 * torch.randint(0, 2, (2, rank, 1), generator=g) - 1)
+    down = torch.zeros((2, rank, 24))
+    down[:, :, [1, 10, 20]] = digits.float() * torch.tensor([65536.0, 256.0, 1.0])
+    up = torch.nn.functional.one_hot(torch.randint(rank, (2, columns), generator=g), rank)
+    x = torch.zeros((rows, 24))
+    x[:, [1, 10, 20]] = 2.0 ** torch.randint(-8, 8, (rows, 1), generator=g)
+    adapters = torch.randint(-1, 2, (rows,), generator=g)
+    adapters[0] = 1
+    s = dict(x=x.bfloat16(), down=down.bfloat16(), up=up.bfloat16(), scale=torch.tensor([1.0, 0.5]), adapters=adapters.int(),
+             into=torch.zeros((rows, columns)), columns=(columns,))
+    assert torch.equal(s["down"].float(), down)
+    want = torch.zeros((rows, columns), dtype=torch.float64)
+    for a in range(2):
+        mine = adapters == a
+        want[mine] = float(s["scale"][a]) * (x[mine].double() @ down[a].double().t()) @ up[a].double().t()
+    assert torch.equal(want.float().double(), want)
+    wrong = (run(ops, s).cpu() != want.float()).nonzero()
+    assert len(wrong) == 0, (len(wrong), wrong[:4].tolist())
