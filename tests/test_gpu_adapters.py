@@ -271,3 +271,83 @@ def test_the_streams_sums_keep_all_bits_of_32(ops, rows, columns, rank):
     assert torch.equal(want.float().double(), want)
     wrong = (run(ops, s).cpu() != want.float()).nonzero()
     assert len(wrong) == 0, (len(wrong), wrong[:4].tolist())
+
+
+def plan_of(ops, s):
+    """The plan that a call of these operands runs, and what it means."""
+    (rows, k), (count, n, rank) = s["x"].shape, s["up"].shape
+    share = 256 // s["x"].element_size()
+    chunk, parts, tile_rows, _slots, block, up_slots = ops.plan_lora(rows, k, n, len(s["columns"]) * rank, rank, count, share, ops.compute_units())
+    chunks = -(-k // chunk)
+    return dict(parts="groups" if parts < chunks else "chunks" if parts > 1 else "one", tile_rows=tile_rows,
+                up="strips" if up_slots == 0 else "rows", steps=-(-rank // (32 if s["x"].element_size() == 2 else 16)))
+
+
+def runs_of(lengths, adapters, rows):
+    """Rows in runs of these lengths, each with the next of these adapters."""
+    out = []
+    while len(out) < rows:
+        out += [adapters[len(out) % len(adapters)]] * lengths[len(out) % len(lengths)]
+    return out[:rows]
+
+
+# rows, k, columns, rank, runs of rows with one adapter: prompts (whole tiles), some dozens of rows (two matrix tiles of an adapter), few
+PROMPTS, DOZENS, FEW = [500, 64, 771], [20, 31, 33, 64], [1, 5, 3, 16, 2]
+FORMS = [
+    # 64-row tiles of the first product, K in chunks or in groups of them, one, two and four column tiles
+    (4032, 4096, (192,), 16, PROMPTS, dict(parts="chunks", tile_rows=64)),
+    (4032, 4096, (192,), 16, DOZENS, dict(parts="chunks", tile_rows=64)),
+    (4100, 4096, (192,), 16, PROMPTS, dict(parts="groups", tile_rows=64)),
+    (6000, 4104, (200,), 28, DOZENS, dict(parts="groups", tile_rows=64)),
+    (2048, 1000, (96, 104), 64, PROMPTS, dict(parts="chunks", tile_rows=64, up="rows")),
+    (2048, 1000, (96, 104), 64, FEW, dict(parts="chunks", tile_rows=64, up="rows")),
+    (2111, 4096, (96, 104), 64, DOZENS, dict(parts="groups", tile_rows=64, up="rows")),
+    (2111, 4096, (96, 104), 100, PROMPTS, dict(parts="groups", tile_rows=64, up="rows")),
+    # the second product's form for many rows, at one, two and four steps of the rank, with whole strips alone, columns behind the last
+    # one, pieces that do not begin on 16 bytes, tiles of one adapter and of many
+    (2111, 4096, (2048, 2560), 64, PROMPTS, dict(parts="groups", tile_rows=64, up="strips")),
+    (2111, 4096, (2100, 2504), 64, DOZENS, dict(parts="groups", tile_rows=64, up="strips")),
+    (2111, 1000, (2048, 2560), 48, FEW, dict(up="strips")),
+    (2111, 1000, (2101, 2555), 64, PROMPTS, dict(up="strips")),
+    (2111, 1000, (2101, 2555), 36, FEW, dict(up="strips")),
+    (2111, 520, (4664,), 44, DOZENS, dict(up="strips")),
+    (2111, 520, (4664,), 20, PROMPTS, dict(up="strips")),
+    (2111, 520, (4663,), 8, PROMPTS, dict(up="strips")),
+]
+
+
+@pytest.mark.parametrize("dtype,stream", KINDS)
+@pytest.mark.parametrize("rows,k,columns,rank,lengths,form", FORMS)
+def test_forms_of_many_rows(ops, dtype, stream, rows, k, columns, rank, lengths, form):
+    s = site(rows, k, columns, rank, 4, getattr(torch, dtype), stream, seed=rows + rank, adapters=runs_of(lengths, [2, 0, -1, 3, 1], rows))
+    plan = plan_of(ops, s)
+    if k > 1000 or dtype == "bfloat16":  # (chunks of float32 are half as long: other parts of a short K)
+        assert {name: plan[name] for name in form} == form
+    check(ops, s)
+    beside = torch.full(s["into"].shape, 9.0, dtype=s["into"].dtype).cuda()
+    assert torch.equal(run(ops, s, out=beside), run(ops, s))
+
+
+def test_the_forms_of_many_rows_are_all_there(ops):
+    seen = set()
+    for dtype, stream in KINDS:
+        for rows, k, columns, rank, _, _ in FORMS:
+            shapes = dict(x=torch.empty((rows, k), dtype=getattr(torch, dtype), device="meta"), up=torch.empty((4, sum(columns), rank)), columns=columns)
+            plan = plan_of(ops, shapes)
+            seen |= {(dtype, plan["parts"], plan["tile_rows"]), (dtype, plan["up"], plan["steps"])}
+    for dtype, steps in (("bfloat16", (1, 2)), ("float32", (1, 2, 3, 4))):
+        assert {(dtype, "chunks", 64), (dtype, "groups", 64), *[(dtype, "strips", s) for s in steps]} <= seen, seen
+
+
+@pytest.mark.parametrize("dtype,stream", KINDS)
+@pytest.mark.parametrize("rows,k,columns,rank", [(2300, 4096, (2100, 2504), 64), (2300, 4104, (2101, 2555), 20), (4200, 11008, (200,), 16),
+                                                 (2300, 4096, (96, 104), 100)])
+def test_a_row_is_the_same_in_every_form(ops, dtype, stream, rows, k, columns, rank):
+    """Bit by bit: a prompt's rows in the forms for many rows, and the same rows alone or with some beside them."""
+    s = site(rows, k, columns, rank, 4, getattr(torch, dtype), stream, seed=rank, adapters=runs_of(PROMPTS, [2, 0, -1, 3, 1], rows))
+    together, plans = run(ops, s).cpu(), {str(plan_of(ops, s))}
+    for first, count in ((0, 1), (63, 2), (rows - 1, 1), (490, 17), (560, 70), (700, 200), (30, 640), (900, 1300)):
+        some = {name: value[first: first + count] if name in ("x", "adapters", "into") else value for name, value in s.items()}
+        plans.add(str(plan_of(ops, some)))
+        assert torch.equal(run(ops, some).cpu(), together[first: first + count]), (first, count, plan_of(ops, some), plan_of(ops, s))
+    assert len(plans) > 1
