@@ -325,3 +325,59 @@ def test_short_lists_of_many_rows_at_once(ops):
     torch.cuda.synchronize()
     for tokens in got:
         assert tokens.tolist() == want
+
+
+@pytest.mark.parametrize("rows,kinds", [(130, "kpm"), (256, "pm"), (256, "p"), (300, "m")])
+def test_rows_of_which_a_workgroup_takes_several_parts(ops, rows, kinds):
+    """So many rows that a launch has fewer workgroups for a row than the row has parts."""
+    vocab = 151936
+    assert ops.RULES_SPREAD // rows < -(-vocab // ops.RULES_PART)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    logits = torch.randn((rows, vocab), generator=g, device="cuda") * torch.linspace(0.3, 4.0, rows, device="cuda")[:, None]
+    logits[::4, 1000:1500] += 6.0
+    h = torch.Generator().manual_seed(rows)
+    pick = lambda values: [values[i] for i in torch.randint(len(values), (rows,), generator=h)]  # noqa: E731
+    uniform = torch.rand(rows, generator=h).tolist()
+    check(ops, logits, pick([0.0, 0.5, 1.0, 1.0, 1.5]), uniform, pick([0, 0, 0, 20, 100]) if "k" in kinds else None,
+          pick([1.0, 0.2, 0.5, 0.9, 0.99, 0.9999]) if "p" in kinds else None, pick([0.0, 0.0, 1e-6, 0.01, 0.3]) if "m" in kinds else None)
+
+
+@pytest.mark.parametrize("vocab", [262145, 1048579, 1100003, (1 << 22) - 1, 1 << 22])
+def test_the_largest_vocabularies(ops, vocab):
+    """More chunks than a row's threads read at once, more parts than a workgroup has threads, and the limit itself.  (Such rows'
+    weights are whole numbers of 2^-40 at the least: none of these, 20 below the largest at most (2^-29), counts as nothing, and
+    their roundings, up to 2^-41 each, add up to some 2^-30 of the largest weight, where a row's sum is thousands of it and a
+    uniform number has 24 bits.)"""
+    assert ops.MAX_RULE_VOCAB == 1 << 22
+    g = torch.Generator().manual_seed(vocab)
+    rows = 8
+    logits = torch.randn((rows, vocab), generator=g).clamp_(-4.0, 4.0) * 1.5
+    logits[1] *= 0.01
+    logits[2, vocab - 70000:] += 8.0
+    logits[3, vocab - 1] = 30.0
+    logits[4, ::3] = -math.inf
+    logits[5, : vocab // 2] = torch.finfo(torch.float32).min
+    logits[6] = torch.randint(0, 3, (vocab,), generator=g).float()
+    uniform = [0.1, 0.5, LAST, 0.3, 0.77, 0.9, 0.25, 0.6]
+    check(ops, logits.cuda(), [1.0] * rows, uniform, [0, 0, 5000, 40, 0, 0, 1000, vocab - 1], [0.9, 0.5, 1.0, 0.9, 0.99, 1.0, 0.9, 0.7],
+          [0.0, 0.0, 0.0, 0.1, 0.0, 0.01, 0.0, 0.0])
+    check(ops, logits.cuda(), [1.0] * rows, uniform, [1, 50, 300, 0, 2000, 20, 0, 0], [1.0, 0.9, 1.0, 1.0, 1.0, 0.5, 0.5, 1.0])
+
+
+def test_refusals_beyond_the_limits(ops):
+    most_rows, most = ops.MAX_RULE_ROWS, ops.MAX_RULE_VOCAB
+    for rows, vocab in ((1, most + 1), (most_rows + 1, 2)):
+        logits, per_row = torch.zeros((rows, vocab)).cuda(), torch.zeros(rows).cuda()
+        with pytest.raises(ValueError):
+            ops.sample(logits, per_row, per_row, top_p=per_row)
+    with pytest.raises(ValueError):
+        ops.token_logprobs(logits, per_row.int())
+    logits, per_row = torch.zeros((most_rows, 2)).cuda(), torch.ones(most_rows).cuda()
+    logits[1::2, 1] = 2.0
+    alternating = [0, 1] * (most_rows // 2) + [0]
+    for rule in (dict(top_k=torch.ones(most_rows, dtype=torch.int32).cuda()), dict(top_p=per_row * 0.0), dict(min_p=per_row)):
+        tokens = ops.sample(logits, per_row, per_row * 0.0, **rule)
+        # (two equal logits: the lower index; one that is larger: that one)
+        assert tokens.tolist() == alternating, list(rule)
+    scores = ops.token_logprobs(logits, tokens).tolist()
+    assert all(abs(score - want) < 1e-6 for score, want in zip(scores, [-math.log(2), -math.log1p(math.exp(-2))] * (most_rows // 2)))
