@@ -11,7 +11,7 @@ import pytest
 import torch
 
 import plain_qwen2 as plain
-from conftest import ROOT, random_tokens
+from conftest import ROOT, TINY, make_folder, random_tokens
 from test_requests_own_cpu import adapter_tensors, write_folder
 
 pytestmark = pytest.mark.gpu
@@ -254,3 +254,54 @@ def test_generate_from_the_command_line(tiny_folders, tmp_path):
     table = log_softmax_of(raw, weights, prompt, tokens)
     scores = json.loads(lines[1])["logprobs"]
     assert len(scores) == 6 and all(math.isfinite(s) and abs(s - table[i, t].item()) < 1e-3 for i, (s, t) in enumerate(zip(scores, tokens)))
+
+
+PROJECTIONS = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj")
+
+
+def check_each_projection(folder, raw, tensors, counts, **options):
+    """A sequence for each projection, with an adapter beside that one alone, and one without any, all in one batch: portions, then
+    captured decode steps.  The engine keeps the stream in float32 and otherwise rounds where the plain model in bfloat16 does, plus
+    the adapter's own sum, so it may be off by twice what that is.  A lost or doubled adapter lies far outside."""
+    from cie_amd.engine.runner import StepEntry
+
+    length = sum(counts)
+    engine = make_engine(folder, dtype="bfloat16", max_adapters=7, token_budget=8 * max(counts), **options)
+    base, slots, whole = float_weights(tensors), {"none": -1}, {"none": random_tokens(length, raw["vocab_size"], 60)}
+    adapters = {}
+    for slot, only in enumerate(PROJECTIONS):
+        factor = 0.3 if only in ("v_proj", "o_proj") else 0.6
+        adapters[only] = {key: t * (factor if ".lora_B." in key else 1.0) for key, t in adapter_tensors(raw, 8, 20 + slot, only).items()}
+        engine.load_adapter(only, tensors=adapters[only], scale=0.8)
+        slots[only], whole[only] = slot, random_tokens(length, raw["vocab_size"], 61 + slot)
+    runner, got, at = engine.runner, {who: [] for who in whole}, 0
+    for who in whole:
+        runner.cache.admit(who)
+    for count in counts:
+        entries = [StepEntry(who, tokens[at: at + count], at, tuple(range(count)), slots[who]) for who, tokens in whole.items()]
+        logits = runner.run(entries).float().cpu().reshape(len(whole), count, -1)
+        for who, rows in zip(whole, logits):
+            got[who].append(rows)
+        at += count
+    assert runner.graphs.adapted_buckets
+    for who, tokens in whole.items():
+        its = [merged(raw, tensors, adapters[who], scale, torch.bfloat16) if slots[who] >= 0 else base for scale in (0.8, 0.0, 1.6)]
+        right, without, twice = (plain.forward(raw, weights, tokens) for weights in its)
+        bound = 2 * (plain.forward(raw, its[0], tokens, dtype=torch.bfloat16).float() - right).abs().max()
+        if slots[who] >= 0:
+            for wrong in (without, twice):
+                assert ((wrong - right).abs() > bound).float().mean() > 0.25, who  # (by the oracle alone)
+        assert (torch.cat(got[who]) - right).abs().max() <= bound, who
+
+
+@pytest.mark.parametrize("name", ["A", "B", "C"])
+def test_each_projections_adapter_in_bfloat16(tiny_folders, name):
+    check_each_projection(*tiny_folders[name], (7, 16, 9, 1, 1, 1, 1, 1, 1, 1, 1))
+
+
+def test_each_projections_adapter_beside_the_wide_models_products(tmp_path):
+    """Widths at which the products take the routes of a model of real size: K cut in parts that are added in no order or summed by
+    the next norm, tiles of many rows, rows that a product would have made the norm of itself."""
+    raw = {**TINY["A"], "hidden_size": 512, "num_attention_heads": 8, "num_key_value_heads": 2, "intermediate_size": 4608}
+    folder, tensors = make_folder(tmp_path, raw, seed=31, factor=1.0)
+    check_each_projection(folder, raw, tensors, (70, 16, 5, 2, 1, 1, 1), kv_tokens=1024)
