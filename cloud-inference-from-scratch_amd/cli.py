@@ -93,8 +93,9 @@ def _make_engine(args: argparse.Namespace):
         options["kv_tokens"] = args.kv_pages * options.get("page_size", EngineConfig.page_size)
     adapter = getattr(args, "adapter", None)
     if adapter:
-        with open(Path(adapter) / "adapter_config.json", encoding="utf-8") as handle:
-            options.update(max_adapters=1, max_adapter_rank=int(json.load(handle).get("r", EngineConfig.max_adapter_rank)))
+        from .engine.adapters import read_config
+
+        options.update(max_adapters=1, max_adapter_rank=read_config(adapter)[0])
     if args.random_weights:
         with open(args.random_weights, encoding="utf-8") as handle:
             config = config_from_dict(json.load(handle))

@@ -16,14 +16,13 @@ from ..parts.adapters import AdapterError, AdapterRoom
 _PREFIX = "base_model.model."
 
 
-def read_adapter(folder: str | Path) -> tuple[dict[str, torch.Tensor], float]:
-    """(tensors by the model's own names, scale) of a folder with ``adapter_config.json`` (``r``, ``lora_alpha``, ``use_rslora``) and
-    ``adapter_model.safetensors``.  What would change the formula and is not built is refused."""
-    import safetensors.torch
-
-    folder = Path(folder)
-    with open(folder / "adapter_config.json", encoding="utf-8") as handle:
+def read_config(folder: str | Path) -> tuple[int, float]:
+    """(rank, scale) of a folder's ``adapter_config.json`` (``r``, ``lora_alpha``, ``use_rslora``).  What would change the formula
+    and is not built is refused."""
+    with open(Path(folder) / "adapter_config.json", encoding="utf-8") as handle:
         raw = json.load(handle)
+    if not isinstance(raw, dict):
+        raise AdapterError("adapter_config.json holds no object")
     faults = []
     if str(raw.get("peft_type", "LORA")).upper() != "LORA":
         faults.append(f"peft_type {raw['peft_type']!r}")
@@ -37,6 +36,15 @@ def read_adapter(folder: str | Path) -> tuple[dict[str, torch.Tensor], float]:
         faults.append(f"r {rank!r} and lora_alpha {alpha!r}")
     if faults:
         raise AdapterError("an adapter of this kind is not run: " + "; ".join(faults))
+    return rank, alpha / (math.sqrt(rank) if raw.get("use_rslora") else rank)
+
+
+def read_adapter(folder: str | Path) -> tuple[dict[str, torch.Tensor], float]:
+    """(tensors by the model's own names, scale) of a folder with ``adapter_config.json`` and ``adapter_model.safetensors``."""
+    import safetensors.torch
+
+    folder = Path(folder)
+    rank, scale = read_config(folder)
     stored = safetensors.torch.load_file(str(folder / "adapter_model.safetensors"))
     tensors = {}
     for name, tensor in stored.items():
@@ -45,7 +53,7 @@ def read_adapter(folder: str | Path) -> tuple[dict[str, torch.Tensor], float]:
     others = sorted({int(t.shape[0]) for name, t in tensors.items() if name.endswith(".lora_A.weight") and t.dim() == 2} - {rank})
     if others:
         raise AdapterError(f"the adapter's r is {rank}, and it has matrices of rank {others}: their scale is not told")
-    return tensors, alpha / (math.sqrt(rank) if raw.get("use_rslora") else rank)
+    return tensors, scale
 
 
 @dataclass(frozen=True)

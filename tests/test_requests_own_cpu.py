@@ -275,3 +275,15 @@ def test_column_blocks_stay_in_a_grids_second_dimension():
                     assert sum(-(-width // block) for width in widths) <= 65535, (n, rows, rank)
                     forms.add(block)
     assert len(forms) > 2 and ops.plan_lora(64, 2048, 22016, 32, 16, 16, 128, 256)[4] == 128  # (as it is for a model's widths)
+
+
+@pytest.mark.parametrize("config", [{"r": None, "lora_alpha": 8}, {"lora_alpha": 8}, {"r": "4", "lora_alpha": 8}, {"r": 4.5, "lora_alpha": 8},
+                                    {"r": 4, "lora_alpha": 8, "use_dora": True}, []])
+def test_the_command_line_refuses_what_the_folder_says(tmp_path, config):
+    """Before an engine is made, and with the refusal that names the fault."""
+    from cie_amd.cli import main
+    from cie_amd.parts.adapters import AdapterError
+
+    folder = write_folder(tmp_path / "a", adapter_tensors(TINY["A"], 4, 7), config)
+    with pytest.raises(AdapterError):
+        main(["generate", "--token-ids", "1 2", "--model", str(tmp_path), "--adapter", str(folder)])
