@@ -29,8 +29,12 @@ def read_config(folder: str | Path) -> tuple[int, float]:
     if raw.get("bias", "none") != "none":
         faults.append(f"bias {raw['bias']!r}")
     faults += [f"{name} {raw[name]!r}" for name in ("use_dora", "fan_in_fan_out", "modules_to_save", "rank_pattern", "alpha_pattern",
-                                                    "lora_bias", "layer_replication", "alora_invocation_tokens")
+                                                    "lora_bias", "layer_replication", "alora_invocation_tokens", "use_qalora",
+                                                    "use_bdlora", "arrow_config")
                if raw.get(name)]
+    # (any other start also takes something out of the weights that the matrices were trained beside)
+    if isinstance(raw.get("init_lora_weights"), str) and raw["init_lora_weights"] not in ("gaussian", "eva", "orthogonal"):
+        faults.append(f"init_lora_weights {raw['init_lora_weights']!r}")
     rank, alpha = raw.get("r"), raw.get("lora_alpha")
     if not (isinstance(rank, int) and rank > 0 and isinstance(alpha, (int, float)) and math.isfinite(alpha)):
         faults.append(f"r {rank!r} and lora_alpha {alpha!r}")

@@ -287,3 +287,20 @@ def test_the_command_line_refuses_what_the_folder_says(tmp_path, config):
     folder = write_folder(tmp_path / "a", adapter_tensors(TINY["A"], 4, 7), config)
     with pytest.raises(AdapterError):
         main(["generate", "--token-ids", "1 2", "--model", str(tmp_path), "--adapter", str(folder)])
+
+
+def test_adapters_trained_beside_other_weights_are_refused(tmp_path):
+    """Starts that move a part of the weights into the matrices leave adapters that are wrong beside the weights themselves."""
+    from cie_amd.engine.adapters import read_adapter
+    from cie_amd.parts.adapters import AdapterError
+
+    tensors = adapter_tensors(TINY["A"], 4, 7)
+    config = {"peft_type": "LORA", "r": 4, "lora_alpha": 6}
+    for fine in (True, False, None, "gaussian", "eva", "orthogonal"):
+        assert read_adapter(write_folder(tmp_path / "a", tensors, {**config, "init_lora_weights": fine}))[1] == 1.5
+    for start in ("pissa", "pissa_niter_16", "olora", "corda", "loftq", "lora_ga"):
+        with pytest.raises(AdapterError):
+            read_adapter(write_folder(tmp_path / "b", tensors, {**config, "init_lora_weights": start}))
+    for change in ({"use_qalora": True}, {"use_bdlora": {"nblocks": 2}}, {"arrow_config": {"top_k": 2}}):
+        with pytest.raises(AdapterError):
+            read_adapter(write_folder(tmp_path / "b", tensors, {**config, **change}))
