@@ -50,10 +50,13 @@ def read_adapter(folder: str | Path) -> tuple[dict[str, torch.Tensor], float]:
     folder = Path(folder)
     rank, scale = read_config(folder)
     stored = safetensors.torch.load_file(str(folder / "adapter_model.safetensors"))
-    tensors = {}
-    for name, tensor in stored.items():
-        name = name[len(_PREFIX):] if name.startswith(_PREFIX) else name
-        tensors[name.replace(".lora_A.default.weight", ".lora_A.weight").replace(".lora_B.default.weight", ".lora_B.weight")] = tensor
+    tensors: dict[str, torch.Tensor] = {}
+    for stored_name, tensor in stored.items():
+        name = stored_name[len(_PREFIX):] if stored_name.startswith(_PREFIX) else stored_name
+        name = name.replace(".lora_A.default.weight", ".lora_A.weight").replace(".lora_B.default.weight", ".lora_B.weight")
+        if name in tensors:
+            raise AdapterError(f"the adapter has {name} under two names")
+        tensors[name] = tensor
     others = sorted({int(t.shape[0]) for name, t in tensors.items() if name.endswith(".lora_A.weight") and t.dim() == 2} - {rank})
     if others:
         raise AdapterError(f"the adapter's r is {rank}, and it has matrices of rank {others}: their scale is not told")

@@ -304,3 +304,15 @@ def test_adapters_trained_beside_other_weights_are_refused(tmp_path):
     for change in ({"use_qalora": True}, {"use_bdlora": {"nblocks": 2}}, {"arrow_config": {"top_k": 2}}):
         with pytest.raises(AdapterError):
             read_adapter(write_folder(tmp_path / "b", tensors, {**config, **change}))
+
+
+def test_a_matrix_under_two_names_is_refused(tmp_path):
+    from cie_amd.engine.adapters import read_adapter
+    from cie_amd.parts.adapters import AdapterError
+
+    tensors = adapter_tensors(TINY["A"], 4, 7)
+    name = next(iter(tensors))
+    for other in (name.replace(".weight", ".default.weight"), "base_model.model." + name):
+        both = {**tensors, other: tensors[name] + 1}
+        with pytest.raises(AdapterError):
+            read_adapter(write_folder(tmp_path / "a", both, {"r": 4, "lora_alpha": 6}, prefix=""))
