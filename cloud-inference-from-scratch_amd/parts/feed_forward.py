@@ -25,6 +25,8 @@ class GatedMLP(Part):
     sums_parts = True  # its last product may come back as parts of K
     takes_adapters = True  # rows of a step may each have a low-rank adapter beside its products
     gates_products = True  # its two products are the SiLU-gate one of ``w_gate_up`` and one of ``w_down``: a block may run them itself
+    site_gate_up: Optional[Site] = None  # (until there is room for adapters)
+
     def __init__(self, hidden_size: int, intermediate_size: int, activation: str = "silu",
                  names: tuple[str, str, str] = ("gate_proj.weight", "up_proj.weight", "down_proj.weight")) -> None:
         if activation != "silu":
@@ -48,7 +50,10 @@ class GatedMLP(Part):
         self.w_down = tensors[prefix + down].contiguous()
 
     def warm_up(self, rows: int) -> None:
-        self.forward(torch.zeros((rows, self.hidden_size), dtype=self.w_down.dtype, device=self.w_down.device))
+        blank = torch.zeros((rows, self.hidden_size), dtype=self.w_down.dtype, device=self.w_down.device)
+        self.forward(blank)
+        if self.site_gate_up is not None:
+            linear(blank, self.w_gate_up)  # (as steps with adapters run it, without the gate: another choice of kernel or algorithm)
 
     def make_sites(self, count: int, rank: int, scale: torch.Tensor) -> dict[str, Module]:
         """Room for adapters beside the two products, by the names of the checkpoint's projections."""

@@ -316,3 +316,27 @@ def test_a_matrix_under_two_names_is_refused(tmp_path):
         both = {**tensors, other: tensors[name] + 1}
         with pytest.raises(AdapterError):
             read_adapter(write_folder(tmp_path / "a", both, {"r": 4, "lora_alpha": 6}, prefix=""))
+
+
+@pytest.mark.parametrize("room", [False, True])
+def test_a_warm_up_runs_the_products_of_steps_with_adapters(monkeypatch, room):
+    """Every product that such a step makes of its rows runs once, in the form in which it makes it, if there is room for adapters."""
+    from cie_amd.parts import attention, feed_forward
+    from cie_amd.parts.adapters import AdapterRoom
+
+    model = model_of(TINY["A"])
+    if room:
+        AdapterRoom(model, 1, 8)
+    ran = []
+
+    def product(x, weight, bias=None, epilogue=None, **_):
+        ran.append((weight.data_ptr(), epilogue))
+        return x.new_zeros((x.shape[0], weight.shape[0] // (2 if epilogue == "silu" else 1)))
+
+    monkeypatch.setattr(attention, "linear", product)
+    monkeypatch.setattr(feed_forward, "linear", product)
+    block = model.blocks[0]
+    block.warm_up(64)
+    mixer, ff = block.mixer, block.feed_forward
+    always = {(w.data_ptr(), None) for w in (mixer.w_qkv, mixer.w_o, ff.w_down)} | {(ff.w_gate_up.data_ptr(), "silu")}
+    assert set(ran) == always | ({(ff.w_gate_up.data_ptr(), None)} if room else set())
