@@ -233,9 +233,21 @@ class Runner:
                  for r in sampling],
                 rules=[r.gen.rules for r in sampling],
             )
-            scores = ops.token_logprobs(logits, on_device) if any(r.gen.logprobs for r in sampling) else None
-            tokens = scored(on_device.tolist(), None if scores is None else scores.cpu())
+            if any(r.gen.logprobs for r in sampling):
+                return self._on_their_way(sampling, logits, on_device).tokens()  # (both are waited for at once)
+            tokens = on_device.tolist()
         return {r.request_id: token for r, token in zip(sampling, tokens)}
+
+    def _on_their_way(self, requests: Sequence[Any], logits: torch.Tensor, tokens: torch.Tensor) -> PendingTokens:
+        """Copies of the requests' drawn tokens, and of their log-probabilities if any asks for them, to the host."""
+        host, scores = torch.empty(len(requests), dtype=torch.int32, pin_memory=True), None
+        host.copy_(tokens, non_blocking=True)
+        if any(r.gen.logprobs for r in requests):
+            scores = torch.empty(len(requests), dtype=torch.float32, pin_memory=True)
+            scores.copy_(ops.token_logprobs(logits, tokens), non_blocking=True)
+        ready = torch.cuda.Event()
+        ready.record()
+        return PendingTokens(tuple(r.request_id for r in requests), host, ready, scores)
 
     # -- decode steps that do not wait for their tokens -----------------------------------
     def can_launch_decode(self, requests: int) -> bool:
@@ -263,15 +275,7 @@ class Runner:
                 [self.sampler.uniform(r.gen.seed, r.serial, index) if r.gen.temperature > 0 else 0.0
                  for r, index in zip(requests, token_indices)],
                 out=pool, rules=[r.gen.rules for r in requests])
-            host = torch.empty(len(requests), dtype=torch.int32, pin_memory=True)
-            host.copy_(pool, non_blocking=True)
-            scores = None
-            if any(r.gen.logprobs for r in requests):
-                scores = torch.empty(len(requests), dtype=torch.float32, pin_memory=True)
-                scores.copy_(ops.token_logprobs(logits, pool), non_blocking=True)
-            ready = torch.cuda.Event()
-            ready.record()
-        return PendingTokens(tuple(r.request_id for r in requests), host, ready, scores)
+            return self._on_their_way(requests, logits, pool)
 
     @property
     def adapter_slots(self) -> int:

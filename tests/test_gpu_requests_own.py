@@ -305,3 +305,26 @@ def test_each_projections_adapter_beside_the_wide_models_products(tmp_path):
     raw = {**TINY["A"], "hidden_size": 512, "num_attention_heads": 8, "num_key_value_heads": 2, "intermediate_size": 4608}
     folder, tensors = make_folder(tmp_path, raw, seed=31, factor=1.0)
     check_each_projection(folder, raw, tensors, (70, 16, 5, 2, 1, 1, 1), kv_tokens=1024)
+
+
+def test_a_step_with_log_probabilities_waits_once(tiny_folders):
+    """Tokens and their log-probabilities travel together: a step that asks for them synchronises no more often than one that
+    does not."""
+    import warnings
+
+    from cie_amd import GenerationConfig
+
+    folder, raw, _ = tiny_folders["A"]
+    engine = make_engine(folder, async_decode=False)
+    waits = {}
+    for logprobs in (False, True):
+        engine.generate([random_tokens(5, raw["vocab_size"], 1)], GenerationConfig(max_output_tokens=4, logprobs=logprobs))
+        with warnings.catch_warnings(record=True) as seen:
+            warnings.simplefilter("always")
+            torch.cuda.set_sync_debug_mode("warn")
+            try:
+                result = engine.generate([random_tokens(6, raw["vocab_size"], 2)], GenerationConfig(max_output_tokens=4, logprobs=logprobs))[0]
+            finally:
+                torch.cuda.set_sync_debug_mode("default")
+        waits[logprobs] = sum("synchronizing" in str(warning.message) for warning in seen)
+    assert len(result.logprobs) == 4 and waits[False] > 0 and waits[True] <= waits[False], waits
