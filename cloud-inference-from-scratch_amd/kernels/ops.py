@@ -11,6 +11,7 @@ from __future__ import annotations
 import contextlib
 import functools
 import math
+import warnings
 
 from typing import Optional
 
@@ -1653,6 +1654,21 @@ def _lora_terms(x_shape, x_strides, dtype, into_shape, into_strides, out_dtype, 
     return rows, *apart, plan[1] * width, numbers + plan, plain, count
 
 
+_SAID_GENERIC: set = set()  # operands whose adapters were sent to the generic kernels, each kind said once
+
+
+def _say_generic(*kind) -> None:
+    if kind in _SAID_GENERIC:
+        return
+    # right, and many times slower than the tiles (2,048 rows of 3,584 to 37,888 at rank 64 15.5 ms, not 0.11): said, not silently
+    _SAID_GENERIC.add(kind)
+    rank, k, apart, misplaced = kind
+    warnings.warn(f"adapters of rank {rank} beside rows of {k} numbers, {apart} apart"
+                  f"{', with x, down or up not on 16 bytes' if misplaced else ''}, take the generic kernels (the matrix-core forms take "
+                  f"ranks that are multiples of 4, and x, down, up and the rows of x in whole pieces of 16 bytes)",
+                  RuntimeWarning, stacklevel=3)
+
+
 def lora_add(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale: torch.Tensor, adapters: torch.Tensor,
              into: torch.Tensor, columns: Optional[tuple] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``out[t] = into[t] + scale[a] * up[a] @ (down[a] @ x[t])`` with ``a = adapters[t]``: every row's own low-rank adapter beside
@@ -1661,7 +1677,8 @@ def lora_add(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale: torch
     x [T, K]; down [A, P * R, K]; up [A, N, R]; scale float32 [A]; adapters int32 [T]; into [T, N] in x's type or float32 (the
     residual stream).  ``columns``: the widths of the P projections that are stacked in the N columns (default: one); projection p
     reads rows p R .. (p + 1) R of ``down``.  ``out`` (default: ``into`` itself) is of into's type.  x, into and out may be views
-    whose rows lie apart; out is ``into`` or shares nothing with any operand.  Sums are float32, rounded once; onto rows of
+    whose rows lie apart; out is ``into`` or shares nothing with any operand.  A rank that is no multiple of 4, or rows of x (or x,
+    down or up themselves) that are not in pieces of 16 bytes take generic kernels, which say so.  Sums are float32, rounded once; onto rows of
     bfloat16 the inner products enter the second sum with 16 bits.  A row's result does not depend on the other rows."""
     dtype, out_dtype = x.dtype, into.dtype
     rows, ldx, ld_into, ld_out, floats, tiled, plain, count = _lora_terms(
@@ -1685,6 +1702,7 @@ def lora_add(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale: torch
     x_at, down_at, up_at = x.data_ptr(), down.data_ptr(), up.data_ptr()
     if tiled is None or (x_at | down_at | up_at) % 16 != 0:  # (a rank, rows or a place that 16-byte loads do not take)
         floats, terms = plain
+        _say_generic(up.shape[2], x.shape[1], ldx, tiled is not None)
     else:
         terms = tiled
     inner = x.new_empty(floats, dtype=torch.float32)

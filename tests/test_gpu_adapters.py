@@ -351,3 +351,26 @@ def test_a_row_is_the_same_in_every_form(ops, dtype, stream, rows, k, columns, r
         plans.add(str(plan_of(ops, some)))
         assert torch.equal(run(ops, some).cpu(), together[first: first + count]), (first, count, plan_of(ops, some), plan_of(ops, s))
     assert len(plans) > 1
+
+
+def test_operands_that_the_matrix_cores_do_not_take_are_told_of(ops, monkeypatch):
+    """Once for each kind: a rank, a length, a distance of the rows, a place; never where the tiles run."""
+    import warnings
+
+    def told(s, **views):
+        with warnings.catch_warnings(record=True) as seen:
+            warnings.simplefilter("always")
+            run(ops, s, **views)
+        return [str(w.message) for w in seen if issubclass(w.category, RuntimeWarning) and "generic kernels" in str(w.message)]
+
+    monkeypatch.setattr(ops, "_SAID_GENERIC", set())
+    fine = site(5, 64, (32,), 8, 2, torch.bfloat16)
+    wide = torch.zeros((5, 80), dtype=torch.bfloat16).cuda()
+    apart = torch.zeros((5, 67), dtype=torch.bfloat16).cuda()
+    assert told(fine) == [] and told(fine, x=wide[:, 8:72]) == []
+    assert told(site(0, 60, (32,), 7, 2, torch.bfloat16)) == []
+    cases = [(site(5, 64, (32,), 6, 2, torch.bfloat16), {}), (site(5, 60, (32,), 8, 2, torch.bfloat16), {}), (fine, dict(x=apart[:, :64])),
+             (fine, dict(x=wide[:, 1:65]))]
+    for s, views in cases:
+        assert len(told(s, **views)) == 1 and told(s, **views) == []
+    assert told(fine) == []
