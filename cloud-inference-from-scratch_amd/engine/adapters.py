@@ -82,8 +82,8 @@ class Adapters:
             raise ValueError("an adapter needs a name")
         if name in self.loaded:
             raise ValueError(f"an adapter {name!r} is loaded already: unload it first")
-        if not math.isfinite(scale):
-            raise ValueError(f"an adapter's scale must be a finite number, not {scale}")
+        if not abs(scale) <= torch.finfo(torch.float32).max:  # (the room holds it in 32 bits)
+            raise ValueError(f"an adapter's scale must be a finite number of 32 bits, not {scale}")
         taken = {known.slot for known in self.loaded.values()}
         slot = next((s for s in range(self.room.count) if s not in taken), None)
         if slot is None:

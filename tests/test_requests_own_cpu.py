@@ -340,3 +340,16 @@ def test_a_warm_up_runs_the_products_of_steps_with_adapters(monkeypatch, room):
     mixer, ff = block.mixer, block.feed_forward
     always = {(w.data_ptr(), None) for w in (mixer.w_qkv, mixer.w_o, ff.w_down)} | {(ff.w_gate_up.data_ptr(), "silu")}
     assert set(ran) == always | ({(ff.w_gate_up.data_ptr(), None)} if room else set())
+
+
+def test_a_scale_that_32_bits_do_not_hold_is_refused():
+    from cie_amd.engine.adapters import Adapters
+    from cie_amd.parts.adapters import AdapterRoom
+
+    adapters = Adapters(AdapterRoom(model_of(TINY["A"]), 1, 8))
+    for scale in (1e39, -1e39, float("nan"), float("-inf")):
+        with pytest.raises(ValueError):
+            adapters.load("one", adapter_tensors(TINY["A"], 4, 3), scale)
+    assert not adapters.loaded
+    adapters.load("one", adapter_tensors(TINY["A"], 4, 3), -3e38)
+    assert torch.isfinite(adapters.room.scale).all()
