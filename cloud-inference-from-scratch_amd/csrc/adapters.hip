@@ -4,15 +4,17 @@
 // projections that read the same rows (q, k and v; gate and up): `down` [A, P R, K] has R rows for each, the columns of `out`
 // fall into P pieces, and p(c) is the piece of column c.
 //
-// The sums are float32, the result is rounded once (h on its way onto rows of bfloat16 keeps 16 bits).  Two launches: `down` (K long, few columns; K cut into parts whose float32 sums
-// lie side by side, so that few rows still fill the GPU) and `up` (R long, many columns; it adds the parts in order).  Rows are
-// taken in tiles of consecutive ones; what a tile does is done once for each adapter that its rows have, on these rows alone,
-// gathered into matrix-core tiles of 16.  So no plan of who has which adapter is made on the host, a row's sums do not depend
-// on its neighbours, and a prompt (one adapter) and 64 requests (16 of them) run through the same code.
+// The sums are float32, the result is rounded once (h on its way onto rows of bfloat16 keeps 16 bits).  Two launches: `down` (K
+// long, few columns; K cut into parts whose float32 sums lie side by side, so that few rows still fill the GPU) and `up` (R long, many
+// columns; it adds the parts in order).  Rows are taken in tiles of consecutive ones; what a tile does is done once for each
+// adapter that its rows have, on these rows alone, gathered into matrix-core tiles of 16.  So no plan of who has which adapter is
+// made on the host, a row's sums do not depend on its neighbours, and a prompt (one adapter) and 64 requests (16 of them) run
+// through the same code.
 //
-// Measured, both products, with what has to be read and written: one row of 2,048 and 2,560 columns, rank 16: 8.2 us (0.3 MB); 64
-// rows of 16 adapters, 2,048 and 22,016, rank 16: 13.9 us (19 MB); 24 rows of 8, 18,944 and 3,584, rank 32: 11.1 us (11.5 MB);
-// 2,048 rows of two, 3,584 and 37,888, rank 64: 110 us (339 MB).
+// Measured in captured chains of calls, both products, with what has to be read and written: one row of 2,048 and 2,560 columns, rank
+// 16: 8.2 us (0.3 MB); 64 rows of 16 adapters, 2,048 and 22,016, rank 16: 12.4 us (19 MB); 24 rows of 8, 18,944 and 3,584, rank 32:
+// 11.1 us (11.5 MB); 2,048 rows of two, 3,584 and 37,888, rank 64: 100 us (339 MB), onto the float32 stream 18,944 and 3,584 94 us.
+// (A kernel's own time under the profiler, which the comments at the kernels give, is some half a us longer, of the last ones a tenth.)
 #include "common.h"
 
 namespace {
@@ -294,7 +296,8 @@ adapter_down_tiles(const T* __restrict__ x, long ldx, const T* __restrict__ down
 
 // The rows of h on their way into the second product, whose result is of type S.  In bfloat16 a number is the sum of several: its
 // rounding, the rounding of what that left out, and so on, 8 bits each, and the product runs once for each.  A float32 stream has all
-// three that a float32 number holds; rows of bfloat16, which keep 8 bits of the sum, two (2^-17 of the number).
+// three that a float32 number holds (with two 92.9 us of 94 for 2,048 rows of 18,944 and 3,584 at rank 64, 0.1 to 0.5 less of smaller
+// ones); rows of bfloat16, which keep 8 bits of the sum, two (2^-17 of the number).
 template <typename T, typename S>
 struct Inner;
 template <typename S>

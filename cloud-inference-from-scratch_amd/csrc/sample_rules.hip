@@ -22,9 +22,9 @@
 // Rows that defeat this (more than kList logits that pass a k's bound, or in the cut's bin) are cut by the bits of their logits.
 //
 // One reading of the logits is what this has to cost; what few rows take beyond it are the launches' chains of small steps (find the
-// largest, add up, sort, add up, cut).  Measured, all launches: one row of 151,936 under top-k and top-p 17 us (0.6 MB; the draw
-// alone 10.6); 8 rows under top-p alone 39 us (4.9 MB; parts 7, tally 9, collect 11, draw 14); 64 rows of all kinds 65 us
-// (38.9 MB; 17, 9, 12, 28); 256 rows of 152,064 under all three rules 62 us (156 MB; parts 27 at 5.7 TB/s, draw 29).  One workgroup
+// largest, add up, sort, add up, cut).  Measured, the kernels' own times: one row of 151,936 under top-k and top-p 18 us (0.6 MB; the
+// draw alone 10.6); 8 rows under top-p alone 41 us (4.9 MB; parts 7, tally 9, collect 11, draw 14); 64 rows of all kinds 64 us
+// (38.9 MB; 17, 9, 11, 28); 256 rows of 152,064 under all three rules 65 us (156 MB; parts 27 at 5.8 TB/s, draw 30).  One workgroup
 // a row for all of it took 282, 400, 459 and 562 us.
 //
 // Every rule keeps a prefix of one order, so what is kept is said by one cut: a logit, and of the tokens that are equal to it

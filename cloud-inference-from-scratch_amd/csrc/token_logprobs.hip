@@ -4,7 +4,7 @@
 // a workgroup each; a row of few is cut in parts, whose pairs a second launch joins in order.  A token outside the vocabulary
 // gives NaN, a row of -inf alone or with a +inf or a NaN gives NaN, as the formula does.
 //
-// What bounds it is the reading: 2,048 rows of 151,936 take 209 us, 5.9 TB/s (a plain reading of 1 GiB 5.6).  8 rows take 6 us for
+// What bounds it is the reading: 2,048 rows of 151,936 take 210 us, 5.9 TB/s (a plain reading of 1 GiB 5.6).  8 rows take 7 us for
 // 4.9 MB, two launches' latency; a workgroup for each whole row takes 31.
 #include "common.h"
 

@@ -92,5 +92,5 @@ class Sampler:
         others = [t for t, on in zip(temperatures, ruled) if not on]
         if any(t > 0 for t in others):
             plain = ops.sample(logits, row[5], row[1])
-            drawn = torch.where(row[0] > 0, drawn, plain)  # (greedy rows are the same in both)
+            drawn = torch.where(row[0] > 0, drawn, plain)  # (greedy rows are the same in both, but those of NaN and -inf alone)
         return drawn if out is None else out.copy_(drawn)
