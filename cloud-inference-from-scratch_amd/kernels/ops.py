@@ -1591,8 +1591,9 @@ MAX_ADAPTER_PIECES = 4
 def plan_lora(rows: int, k: int, n: int, inner: int, rank: int, count: int, share: int, units: int) -> tuple[int, int, int, int, int, int]:
     """(k of a chunk, parts, rows of a tile of the first product, workgroups for a tile's adapters, columns of a workgroup of the
     second product, workgroups for the adapters of its 64 rows) of :func:`lora_add`.  ``share``: the k that a workgroup takes at
-    a time.  Times: both products in us, in captured chains of calls, each pair from one run.  64 rows are decoding rows of 16 adapters of rank 16 (K 2,048, 22,016 columns), 24 of
-    8 of rank 32 (18,944, 3,584), 618 a batch with prompts (2,048, 2,560); 2,048 rows are two prompts (3,584, 37,888, rank 64)."""
+    a time.  Times: both products in us, in captured chains of calls, each pair from one run.  64 rows are decoding rows of 16
+    adapters of rank 16 (K 2,048, 22,016 columns), 24 of 8 of rank 32 (18,944, 3,584), 618 a batch with prompts (2,048, 2,560);
+    2,048 rows are two prompts (3,584, 37,888, rank 64)."""
     # up to 16 chunks, by K alone, so that the sums are the same whatever rows come along (24 rows: 8 chunks 13.1, 15 11.1, 25 12.2)
     chunk = max(1, -(-k // (32 * share))) * 2 * share
     chunks = -(-k // chunk)
